@@ -17,6 +17,9 @@ SRC_PATH = os.path.join(_HERE, "csrc", "loops_c_abi.hip")
 PROBES_LIB_PATH = os.environ.get("LOOPS_PROBES_LIB", os.path.join(_HERE, "libloops_probes.so"))
 PROBES_SRC_PATH = os.path.join(_HERE, "csrc", "loops_probes.hip")
 INCLUDE_DIR = os.path.join(_ROOT, "include")
+# no packed fp32 instructions (v_pk_add_f32 and its like, which -O3 makes from ordinary float code): some of their forms have given
+# wrong results on gfx950 now and then.  (hipcc's host pass warns that it does not know the feature.)
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # enum loops_schedule (include/loops_amd.h)
 MERGE_PATH_FLAT, WORK_ORIENTED, THREAD_MAPPED, GROUP_MAPPED, ORIGINAL, FLAT_PARTITIONED = range(6)
@@ -89,13 +92,13 @@ def _compile(src: str, out: str, extra_deps=(), force: bool = False, verbose: bo
     deps = [src, *extra_deps]
     for base, _, files in os.walk(INCLUDE_DIR):
         deps += [os.path.join(base, f) for f in files]
-    digest = source_digest(deps) + " " + " ".join(sorted(defines))
+    digest = source_digest(deps) + " " + " ".join([*DEVICE_FLAGS, *sorted(defines)])
     stamp = out + ".srcdigest"
     force = force or os.environ.get("LOOPS_FORCE_BUILD", "0") not in ("", "0")
     if not force and os.path.exists(out) and os.path.exists(stamp) and open(stamp).read().strip() == digest.strip():
         return out
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-DLOOPS_TARGET_GFX=0x950",
+    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-DLOOPS_TARGET_GFX=0x950", *DEVICE_FLAGS,
            *["-D" + d for d in defines], "-I" + INCLUDE_DIR, src, "-o", out]
     if verbose:
         print(" ".join(cmd))
