@@ -572,6 +572,66 @@ const char* loops_comm_error_string(int code);
 int loops_allgatherv_f32(void* comm, int rank, int world, float* y_full, const long long* bounds, void* stream);
 int loops_allgatherv_f64(void* comm, int rank, int world, double* y_full, const long long* bounds, void* stream);
 
+/* ---- embedding of tokens ---------------------------------------------------------------------------------------------------
+ * No reference counterpart.  The products of a token matrix (tokens x rows of a table, one 1 per token) with the table and of its
+ * transpose with the gradient of the result: the SpMM of this library where the sparse operand is a list of ids
+ * (include/loops/kernels/embedding.hxx, group_ids.hxx).
+ * Values are float, half or bfloat16 (enum loops_value_type), ids are int or long long (enum loops_index_type); another number
+ * returns LOOPS_E_CONFIG.  Matrices are row-major with unit column stride; a pitch is the distance of two rows in elements (>= the
+ * row's width, LOOPS_E_BADARG otherwise), at any alignment of the element.  No output may overlap an input.
+ * `first_id` (>= 0): the id of the table's row 0.  A token whose id is outside [first_id, first_id + rows) -- padding, or a row that
+ * another rank's shard of the table holds -- has a zero row in the lookup and no part in the gradient; no id is an error.
+ * Calls are asynchronous and may be captured; they keep nothing between calls: scratch memory is the caller's `workspace`
+ * (hipMalloc'd, 16-byte aligned, at least what the *_workspace function says for the same sizes, LOOPS_E_BADARG otherwise; it may be
+ * NULL where that is 0), used by one call at a time.  tokens + rows must stay below 2^31 (LOOPS_E_RANGE). */
+enum loops_value_type { LOOPS_VALUE_F32 = 0, LOOPS_VALUE_F16 = 1, LOOPS_VALUE_BF16 = 2 };
+enum loops_index_type { LOOPS_INDEX_I32 = 0, LOOPS_INDEX_I64 = 1 };
+
+/* out[t, :] = scale * table[id_t - first_id, :], the product in float, rounded once.  The table and `out` have `value_type`. */
+int loops_embedding_lookup(int value_type, int index_type, int rows, int dim, const void* table, long long table_pitch, int tokens,
+                           const void* token_ids, long long first_id, float scale, void* out, long long out_pitch, void* stream);
+
+/* Positions grouped by id: ids[0 .. tokens) = id - first_id in ascending order, positions[i] = where ids[i] stands in `token_ids`,
+ * ascending within equal ids (a stable sort).  Tokens without a row -- out of range, or equal to `drop_id` (-1: none) -- have
+ * ids[i] = rows and so stand behind all others.  Also orders (token, choice) pairs of a router by expert. */
+int loops_group_tokens_workspace(int tokens, int rows, size_t* bytes);
+int loops_group_tokens(int index_type, int tokens, const void* token_ids, int rows, long long first_id, long long drop_id, int* ids,
+                       int* positions, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[v, :] = scale * sum of grad[positions[i], :] over ids[i] = v, sums in float, rounded once; `ids` / `positions` as
+ * loops_group_tokens wrote them for these tokens and rows.  accumulate = 0: every row of `out` is written (zeros where there is no
+ * token); otherwise the sums are added to what rows with tokens hold and the other rows are left as they are.  `out` has `grad_type`
+ * or is float (LOOPS_E_CONFIG otherwise).  The order of summation is fixed: equal inputs give equal bits. */
+int loops_embedding_gradient_workspace(int grad_type, int tokens, int rows, int dim, int accumulate, size_t* bytes);
+int loops_embedding_gradient(int grad_type, int out_type, int tokens, const int* ids, const int* positions, int rows, int dim,
+                             const void* grad, long long grad_pitch, float scale, int accumulate, void* out, long long out_pitch,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- balance of a router ---------------------------------------------------------------------------------------------------
+ * No reference counterpart.  Column sums of the routing matrix (tokens x experts, `choices` ones per row) and the loss that keeps
+ * them even (include/loops/kernels/balance_loss.hxx).  Types, pitches, workspaces and capture as above.  1 <= experts <= 1024
+ * (LOOPS_E_CONFIG beyond), tokens * choices < 2^31 (LOOPS_E_RANGE).  `chosen` [tokens, choices]: expert indices, packed; indices outside
+ * [0, experts) are not counted.  `mask` [tokens] (NULL: all): a token whose byte is 0 takes no part in anything and its gradient row is 0
+ * (its logits may hold anything). */
+int loops_expert_counts_workspace(int tokens, int choices, int experts, size_t* bytes);
+int loops_expert_counts(int index_type, int tokens, int choices, const void* chosen, const unsigned char* mask, int experts, int* counts,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* With p = softmax(logits) per token, n the number of tokens that take part, c = the counts:
+ *   counts[e] = c_e,  probability[e] = mean of p_e over the n tokens,  *counted_tokens = n,
+ *   *loss = coefficient * experts * sum_e c_e / (n * choices) * probability[e]      (0 where n = 0)
+ * A row of logits that are all -infinity has p = 0 (and counts in n).
+ * Backward: grad = *grad_loss (NULL: 1) * d loss / d logits, the counts taken as constants:
+ *   coefficient * experts / n * p_e * (f_e - sum_j f_j p_j),  f = c / (n * choices).
+ * `counts` and `counted_tokens` as the forward call wrote them; `grad` has the logits' type. */
+int loops_balance_loss_workspace(int tokens, int experts, size_t* bytes);
+int loops_balance_loss(int value_type, int index_type, int tokens, int experts, int choices, const void* logits, long long logits_pitch,
+                       const void* chosen, const unsigned char* mask, float coefficient, float* loss, int* counts, float* probability,
+                       int* counted_tokens, void* workspace, size_t workspace_bytes, void* stream);
+int loops_balance_loss_backward(int value_type, int tokens, int experts, int choices, const void* logits, long long logits_pitch,
+                                const int* counts, const int* counted_tokens, const unsigned char* mask, float coefficient,
+                                const float* grad_loss, void* grad, long long grad_pitch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,8 @@ SYMBOLS = [
     "loops_bcsr_band_plan_create_f32", "loops_bcsr_band_plan_destroy", "loops_bcsr_band_plan_info", "loops_bcsr_band_plan_arrays",
     "loops_bcsr_band_plan_set_chunks", "loops_bcsr_band_plan_tune", "loops_bcsr_band_plan_set_shape", "loops_bcsr_band_plan_refresh_values_f32",
     "loops_spmv_bcsr_band_f32", "loops_spmv_bcsr_band_stage_f32",
+    "loops_embedding_lookup", "loops_group_tokens_workspace", "loops_group_tokens", "loops_embedding_gradient_workspace", "loops_embedding_gradient",
+    "loops_expert_counts_workspace", "loops_expert_counts", "loops_balance_loss_workspace", "loops_balance_loss", "loops_balance_loss_backward",
 ]
 
 
@@ -262,11 +264,22 @@ def lib() -> C.CDLL:
         L.loops_autotune_merge_path_variants_f32.argtypes = [ci, ci, ci, vp, vp, vp, vp, vp, ci, vp, C.POINTER(ci), C.POINTER(ci), vp]
         L.loops_spmv_plan_variant.argtypes = [vp, C.POINTER(ci), C.POINTER(C.c_float)]
         L.loops_columns_look_scattered.argtypes = [ci, ci, vp, ci, vp, C.POINTER(ci)]
+        cll, cf, size = C.c_longlong, C.c_float, C.c_size_t
+        L.loops_embedding_lookup.argtypes = [ci, ci, ci, ci, vp, cll, ci, vp, cll, cf, vp, cll, vp]
+        L.loops_group_tokens_workspace.argtypes = [ci, ci, C.POINTER(size)]
+        L.loops_group_tokens.argtypes = [ci, ci, vp, ci, cll, cll, vp, vp, vp, size, vp]
+        L.loops_embedding_gradient_workspace.argtypes = [ci, ci, ci, ci, ci, C.POINTER(size)]
+        L.loops_embedding_gradient.argtypes = [ci, ci, ci, vp, vp, ci, ci, vp, cll, cf, ci, vp, cll, vp, size, vp]
+        L.loops_expert_counts_workspace.argtypes = [ci, ci, ci, C.POINTER(size)]
+        L.loops_expert_counts.argtypes = [ci, ci, ci, vp, vp, ci, vp, vp, size, vp]
+        L.loops_balance_loss_workspace.argtypes = [ci, ci, C.POINTER(size)]
+        L.loops_balance_loss.argtypes = [ci, ci, ci, ci, ci, vp, cll, vp, vp, cf, vp, vp, vp, vp, vp, size, vp]
+        L.loops_balance_loss_backward.argtypes = [ci, ci, ci, ci, vp, cll, vp, vp, vp, cf, vp, vp, cll, vp]
         _lib = L
     return _lib
 
 
-_ERRORS = {-1: "LOOPS_E_BADARG", -2: "LOOPS_E_RANGE (rows + nnz must stay below 2^31)", -3: "LOOPS_E_CONFIG"}
+_ERRORS = {-1: "LOOPS_E_BADARG", -2: "LOOPS_E_RANGE (rows + nnz must stay below 2^31)", -3: "LOOPS_E_CONFIG"}  # (the same sum for tokens + rows)
 
 
 def check(code: int, what: str) -> None:

@@ -4,7 +4,7 @@
 // index_t = offset_t = int, type_t = float | double and launches them on the caller's
 // stream.  No CPU fallbacks live here: if a kernel cannot be launched the hipError_t is
 // returned.  Built by __graft_entry__.build() with
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -Iinclude loops_c_abi.hip
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude loops_c_abi.hip
 #include <loops_amd.h>
 
 #include <algorithm>
@@ -34,6 +34,8 @@
 #include <loops/kernels/bcsr_spmv.hxx>
 #include <loops/kernels/bcsr_band.hxx>
 #include <loops/kernels/bcsr_merge_path.hxx>
+#include <loops/kernels/embedding.hxx>
+#include <loops/kernels/balance_loss.hxx>
 
 using namespace loops;
 using kernels::coord_t;
@@ -79,3 +81,5 @@ inline int check_csr(int rows, int cols, int nnz, const void* off, const void* i
 #include "abi_bcsr_band.inc"
 #include "abi_plans.inc"
 #include "abi_multi_gpu.inc"
+#include "abi_embedding.inc"
+#include "abi_routing.inc"

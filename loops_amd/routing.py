@@ -1,0 +1,98 @@
+"""Tokens per expert and the balance loss of a router, with its gradient, over the C ABI (``loops_expert_counts``,
+``loops_balance_loss*``): column sums of a routing matrix (tokens x experts, ``choices`` ones per row).
+
+With p = softmax(logits), c the counts, n the number of tokens whose mask holds and k the choices per token::
+
+    loss = coefficient * experts * sum_e c_e / (n k) * mean_t p_te
+
+The order in which experts take their tokens is ``embedding.group_tokens(chosen, experts)``.  Logits are float32, float16 or bfloat16,
+expert indices int32 or int64 (one outside [0, experts) is not counted).  Calls are asynchronous on the current stream of the tensors'
+device and may be captured into a graph; there is no CPU path.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .embedding import index_type, launch, overlap, pitch_of, require, same_device, value_type, workspace
+
+
+def _mask(mask: Optional[torch.Tensor], tokens: int):
+    if mask is None:
+        return None
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise TypeError("mask must be bool or uint8")
+    require(mask.is_contiguous() and mask.numel() == tokens, "mask must be contiguous with an element for each token")
+    return mask.data_ptr()
+
+
+def expert_counts(chosen: torch.Tensor, experts: int, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """int32 [experts]: how often each expert stands in ``chosen`` ([tokens, choices] or [tokens], contiguous), in the rows whose
+    ``mask`` holds."""
+    index = index_type(chosen, "chosen")
+    require(chosen.dim() in (1, 2) and chosen.is_contiguous(), "chosen must be [tokens, choices], contiguous")
+    tokens = chosen.shape[0]
+    choices = chosen.shape[1] if chosen.dim() == 2 else 1
+    device = same_device(chosen, mask)
+    masked = _mask(mask, tokens)
+    _keep, ws, size = workspace(device, "loops_expert_counts_workspace", tokens, choices, experts)
+    counts = torch.empty(experts, dtype=torch.int32, device=device)
+    launch(device, "loops_expert_counts", index, tokens, choices, chosen.data_ptr(), masked, experts, counts.data_ptr(), ws, size)
+    return counts
+
+
+class BalanceLoss(NamedTuple):
+    """What ``balance_loss`` found; ``balance_loss_backward`` takes it back."""
+    loss: torch.Tensor         # float32 []
+    counts: torch.Tensor       # int32 [experts]
+    probability: torch.Tensor  # float32 [experts]: mean over the tokens that take part
+    tokens: torch.Tensor       # int32 []: how many those are
+    choices: int
+    coefficient: float
+
+
+def balance_loss(logits: torch.Tensor, chosen: torch.Tensor, coefficient: float = 1.0, mask: Optional[torch.Tensor] = None) -> BalanceLoss:
+    """The balance loss of ``logits`` [tokens, experts] (any distance between rows) for the experts ``chosen`` [tokens, choices] (contiguous);
+    ``mask`` [tokens]: the tokens that take part (all where it is None)."""
+    value, index = value_type(logits, "logits"), index_type(chosen, "chosen")
+    pitch = pitch_of(logits, "logits")
+    tokens, experts = logits.shape
+    require(chosen.dim() == 2 and chosen.shape[0] == tokens and chosen.is_contiguous(), "chosen must be [tokens, choices], contiguous")
+    choices = chosen.shape[1]
+    device = same_device(logits, chosen, mask)
+    masked = _mask(mask, tokens)
+    _keep, ws, size = workspace(device, "loops_balance_loss_workspace", tokens, experts)
+    whole = torch.empty(experts + 1, dtype=torch.int32, device=device)
+    real = torch.empty(experts + 1, dtype=torch.float32, device=device)
+    at_whole, at_real = whole.data_ptr(), real.data_ptr()
+    launch(device, "loops_balance_loss", value, index, tokens, experts, choices, logits.data_ptr(), pitch, chosen.data_ptr(), masked, coefficient,
+           at_real + 4 * experts, at_whole, at_real, at_whole + 4 * experts, ws, size)
+    return BalanceLoss(real[experts], whole[:experts], real[:experts], whole[experts], choices, coefficient)
+
+
+def balance_loss_backward(logits: torch.Tensor, forward: BalanceLoss, mask: Optional[torch.Tensor] = None, grad_loss: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``grad_loss * loss`` (a float32 scalar on the device; 1 where it is None) with respect to ``logits``, in their type: [tokens,
+    experts].  ``logits`` and ``mask`` as in the forward call, ``forward`` what it returned."""
+    value = value_type(logits, "logits")
+    pitch = pitch_of(logits, "logits")
+    tokens, experts = logits.shape
+    require(forward.counts.shape == (experts,), "forward was made of another number of experts")
+    device = same_device(logits, forward.counts, forward.tokens, mask, grad_loss, out)
+    masked = _mask(mask, tokens)
+    upstream = None
+    if grad_loss is not None:
+        if grad_loss.dtype is not torch.float32:
+            raise TypeError("grad_loss must be float32")
+        require(grad_loss.numel() == 1, "grad_loss must be a scalar")
+        upstream = grad_loss.data_ptr()
+    if out is None:
+        out = torch.empty(tokens, experts, dtype=logits.dtype, device=device)
+    else:
+        require(out.dtype is logits.dtype and out.shape == logits.shape, "out must have the logits' shape and type")
+        require(not overlap(out, logits) and not overlap(out, forward.counts) and not overlap(out, forward.tokens) and
+                (mask is None or not overlap(out, mask)) and (grad_loss is None or not overlap(out, grad_loss)), "out must not overlap the inputs")
+    launch(device, "loops_balance_loss_backward", value, tokens, experts, forward.choices, logits.data_ptr(), pitch, forward.counts.data_ptr(),
+           forward.tokens.data_ptr(), masked, forward.coefficient, upstream, out.data_ptr(), pitch_of(out, "out"))
+    return out
