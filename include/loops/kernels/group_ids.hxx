@@ -4,12 +4,13 @@
  * position (row = position, column = id).  What the embedding gradient sums over and what experts' products are dispatched by.
  *
  * key(i) = id_i - first for ids in [first, first + rows) other than `drop`, `rows` otherwise (those end up behind the last group).
- * Least-significant-digit radix sort, digits of at most 10 bits, ceil(log2(rows + 1) / digits) of them:
  *
- *   n <= 8 192   ONE workgroup keeps keys and positions in LDS through all passes: one launch.
- *   beyond       two launches a pass.  COUNT: workgroup w counts the digits of its span (n / W consecutive items, W <= 256).  PLACE:
- *                every workgroup adds the counts of the spans before it by itself (W x digits words from L2; no scan launch), then each
- *                of its 16 wavefronts counts and places its own sixteenth of the span.
+ *   n <= 8 192   RANK, one launch: an item's place is the number of items that come before it.  Every workgroup holds all keys in LDS and
+ *                finds the places of 16 items: n^2 comparisons over the whole chip, whatever the ids.
+ *   beyond       least-significant-digit radix sort, digits of at most 10 bits, ceil(log2(rows + 1) / digits) of them, two launches each.
+ *                COUNT: workgroup w counts the digits of its span (n / W consecutive items, W <= 128).  PLACE: every workgroup adds up the
+ *                counts of the spans before it (W x digits words from L2; no scan launch), then each of its 16 wavefronts counts and
+ *                places its own sixteenth of the span.
  *
  * A wavefront ranks 64 items at a time without atomics: one ballot per digit bit leaves each lane the mask of the lanes with its digit;
  * the rank is the number of mask bits below the lane and the last of them advances the wavefront's counter in LDS.  Items are taken in
@@ -17,9 +18,9 @@
  */
 #pragma once
 
-#include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <type_traits>
 
 #include <hip/hip_runtime.h>
 
@@ -33,8 +34,8 @@ constexpr int threads = 1024;
 constexpr int waves = threads / wave::size;
 constexpr int max_digit_bits = 10;
 constexpr int max_digits = 1 << max_digit_bits;
-constexpr int block_items = 8192;  ///< what one workgroup sorts in LDS
-constexpr int max_spans = 256;
+constexpr int rank_items = 8192;  ///< most items of the RANK form
+constexpr int max_spans = 128;
 
 /// Which ids count, and what they become.
 struct key_map {
@@ -55,37 +56,36 @@ struct item_t {
 };
 
 struct plan_t {
-  int passes;
-  int bits;   ///< per digit
-  int spans;  ///< workgroups of a COUNT / PLACE launch (1: everything in one workgroup)
-  int span;   ///< items per workgroup
+  int passes;  ///< 0: RANK
+  int bits;    ///< per digit
+  int spans;   ///< workgroups of a launch
+  int span;    ///< items per workgroup
 };
 
-/// Bits are shared out evenly: 18 bits are two digits of 9.  A span is at least 4 096 items (four rounds per wavefront) and there
-/// are at most 256, so that the counts a PLACE workgroup adds up stay within 1 MB.
+/// Bits are shared out evenly: 18 bits are two digits of 9.  A span is 1 024 items (one per thread) until there would be more than 128.
 inline plan_t plan_for(int n, int rows) {
-  int bits = 1;
+  plan_t p{0, 0, 0, 0};
+  if (n <= rank_items) return p;
+  int bits = 2;
   while (bits < 31 && (static_cast<unsigned int>(rows) >> bits) != 0u) ++bits;
-  plan_t p;
   p.passes = (bits + max_digit_bits - 1) / max_digit_bits;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.spans = 1;
-  p.span = n;
-  if (n > block_items) {
-    const int want = (n + 4095) / 4096;
-    const int w = want < max_spans ? want : max_spans;
-    const long long per = (static_cast<long long>(n) + w - 1) / w;
-    p.span = static_cast<int>((per + threads - 1) / threads * threads);
-    p.spans = static_cast<int>((static_cast<long long>(n) + p.span - 1) / p.span);
-  }
+  const int want = (n + threads - 1) / threads;
+  const int w = want < max_spans ? want : max_spans;
+  const long long per = (static_cast<long long>(n) + w - 1) / w;
+  p.span = static_cast<int>((per + threads - 1) / threads * threads);
+  p.spans = static_cast<int>((static_cast<long long>(n) + p.span - 1) / p.span);
   return p;
 }
 
+inline std::size_t item_bytes(int n) { return (static_cast<std::size_t>(n) * sizeof(item_t) + 255) & ~static_cast<std::size_t>(255); }
+
+/// Items between the passes (two buffers in turn), counts[spans][digits].
 inline std::size_t workspace_bytes(int n, int rows) {
   const plan_t p = plan_for(n, rows);
-  if (p.spans == 1) return 0;
-  const std::size_t items = (static_cast<std::size_t>(n) * sizeof(item_t) + 255) & ~static_cast<std::size_t>(255);
-  return items * static_cast<std::size_t>(p.passes > 2 ? 2 : p.passes - 1) + static_cast<std::size_t>(p.spans) * (static_cast<std::size_t>(1) << p.bits) * sizeof(int);
+  if (p.passes == 0) return 0;
+  return item_bytes(n) * static_cast<std::size_t>(p.passes > 2 ? 2 : p.passes - 1) +
+         static_cast<std::size_t>(p.spans) * (static_cast<std::size_t>(1) << p.bits) * sizeof(int);
 }
 
 namespace detail {
@@ -152,89 +152,53 @@ __device__ __forceinline__ void places(int* __restrict__ s_count, int digits, in
 
 }  // namespace detail
 
-/// n <= IPT * 1 024 items, all passes in one workgroup.  Item j of wavefront w, lane l is w * 64 * IPT + j * 64 + l.
-template <int IPT, typename id_t>
+constexpr int rank_group = 16;                                 ///< items per workgroup of `rank`
+constexpr int rank_parts = threads / rank_group;               ///< threads per item
+
+/// Workgroup b finds the places of items [16 b, 16 b + 16).  Thread (part, item) compares its item with every 64th group of 4 keys, so
+/// that a wavefront's LDS read fetches 16 keys for 16 items each.
+template <typename id_t>
 __global__ void __launch_bounds__(threads)
-sort_block(const int n, const id_t* __restrict__ in, const key_map map, const int passes, const int bits, int* __restrict__ ids,
-           int* __restrict__ positions) {
-  extern __shared__ int s_mem[];
-  const int digits = 1 << bits;
-  int* const s_scan = s_mem;                // [16]
-  int* const s_count = s_mem + waves;       // [waves][digits]
-  unsigned int* const s_key = reinterpret_cast<unsigned int*>(s_count + waves * digits);  // [n]
-  int* const s_position = reinterpret_cast<int*>(s_key + IPT * threads);                  // [n]
+rank(const int n, const id_t* __restrict__ in, const key_map map, int* __restrict__ ids, int* __restrict__ positions) {
+  typedef unsigned int quad_t __attribute__((ext_vector_type(4)));
+  __shared__ quad_t s_key[rank_items / 4];
+  __shared__ int s_before[waves][rank_group];
   const int tid = threadIdx.x;
-  const int w = tid / wave::size;
-  const int first = w * wave::size * IPT + wave::lane();
-  int* const mine = s_count + w * digits;
-
-  unsigned int key[IPT];
-  int position[IPT];
-#pragma unroll
-  for (int j = 0; j < IPT; ++j) {
-    const int i = first + j * wave::size;
-    position[j] = i;
-    key[j] = i < n ? map(in[i]) : 0u;
+  const int quads = (n + 3) / 4;
+  unsigned int* const keys = reinterpret_cast<unsigned int*>(s_key);
+  for (int i = tid; i < quads * 4; i += threads) keys[i] = i < n ? map(in[i]) : 0xFFFFFFFFu;  // (behind every key)
+  __syncthreads();
+  const int first = static_cast<int>(blockIdx.x) * rank_group;
+  const int mine = first + tid % rank_group;
+  const int part = tid / rank_group;
+  const unsigned int key = keys[mine < n ? mine : 0];
+  int before = 0;
+  const int own = first / 4, behind = own + rank_group / 4;
+#pragma unroll 4
+  for (int q = part; q < own; q += rank_parts) {
+    const quad_t k = s_key[q];
+    before += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
   }
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * bits;
-    for (int i = tid; i < waves * digits; i += threads) s_count[i] = 0;
-    __syncthreads();
-    int rank[IPT];  // among the wavefront's items of the digit
-#pragma unroll
-    for (int j = 0; j < IPT; ++j)
-      rank[j] = detail::take(mine, (key[j] >> shift) & (digits - 1), bits, first + j * wave::size < n);
-    __syncthreads();
-    int total = 0;
-    if (tid < digits)
-      for (int v = 0; v < waves; ++v) total += s_count[v * digits + tid];
-    const int base = detail::block_exclusive_sum(total, s_scan);
-    detail::places(s_count, digits, base);
-    __syncthreads();
-    const bool last = pass == passes - 1;
-#pragma unroll
-    for (int j = 0; j < IPT; ++j) {
-      if (first + j * wave::size < n) {
-        const int at = mine[(key[j] >> shift) & (digits - 1)] + rank[j];
-        if (last) {
-          ids[at] = static_cast<int>(key[j]);
-          positions[at] = position[j];
-        } else {
-          s_key[at] = key[j];
-          s_position[at] = position[j];
-        }
-      }
-    }
-    if (!last) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < IPT; ++j) {
-        const int i = first + j * wave::size;
-        if (i < n) {
-          key[j] = s_key[i];
-          position[j] = s_position[i];
-        }
-      }
-      __syncthreads();
-    }
+#pragma unroll 4
+  for (int q = behind + part; q < quads; q += rank_parts) {
+    const quad_t k = s_key[q];
+    before += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
   }
-}
-
-/// sort_block's launch.  Its LDS is up to 128 KB (10-bit digits, 8 192 items): beyond 64 KB a kernel is opted in once per device.
-template <int IPT, typename id_t>
-void launch_sort_block(hipStream_t stream, int n, const id_t* in, const key_map& map, const plan_t& p, int* ids, int* positions) {
-  static std::atomic<unsigned long long> opted{0ull};
-  const std::size_t items = p.passes > 1 ? 2u * IPT * threads : 0u;
-  const std::size_t lds = sizeof(int) * (waves + static_cast<std::size_t>(waves) * (static_cast<std::size_t>(1) << p.bits) + items);
-  if (lds > 64 * 1024) {
-    int device = 0;
-    const bool known = hipGetDevice(&device) == hipSuccess && device >= 0 && device < 64;
-    if (!known || !((opted.load() >> device) & 1ull)) {
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&sort_block<IPT, id_t>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-      if (known) opted.fetch_or(1ull << device);
-    }
+  if (part < rank_group) {  // the workgroup's own 16: equal keys in the order of their positions
+    const int j = first + part;
+    if (j < n) before += keys[j] < key || (keys[j] == key && j < mine);
   }
-  sort_block<IPT, id_t><<<1, threads, lds, stream>>>(n, in, map, p.passes, p.bits, ids, positions);
+#pragma unroll
+  for (int d = rank_group; d < wave::size; d <<= 1) before += __shfl_xor(before, d, wave::size);
+  if (wave::lane() < rank_group) s_before[tid / wave::size][wave::lane()] = before;
+  __syncthreads();
+  if (tid < rank_group && mine < n) {
+    int place = 0;
+#pragma unroll
+    for (int i = 0; i < waves; ++i) place += s_before[i][tid];
+    ids[place] = static_cast<int>(key);
+    positions[place] = mine;
+  }
 }
 
 /// Item i of the pass's input: raw ids on the first pass, items afterwards.
@@ -268,17 +232,46 @@ __global__ void __launch_bounds__(threads)
 place_digits(const int n, const id_t* __restrict__ raw, const item_t* __restrict__ items, const key_map map, const int shift, const int bits,
              const int span, const int spans, const int* __restrict__ counts, item_t* __restrict__ out, int* __restrict__ ids,
              int* __restrict__ positions) {
+  typedef int quad_t __attribute__((ext_vector_type(4)));
   __shared__ int s_scan[waves];
-  __shared__ int s_count[waves * max_digits];
+  __shared__ quad_t s_quad[waves * max_digits / 4];
+  int* const s_mem = reinterpret_cast<int*>(s_quad);
   const int digits = 1 << bits;
   const int tid = threadIdx.x;
   const int w = tid / wave::size;
+
+  // the place of the workgroup's first item of digit `tid`: items of lower digits, and of the digit in earlier spans.  A thread adds up
+  // 4 digits, the spans dealt out to slices of the threads; digits above the largest key's are left out
+  const unsigned int top = static_cast<unsigned int>(map.rows) >> shift;
+  const int quads = top < static_cast<unsigned int>(digits) ? static_cast<int>(top) / 4 + 1 : digits / 4;
+  const int slices = threads / quads;
+  const int slice = tid / quads, quad = tid % quads;
+  if (slice < slices) {
+    quad_t before = {0, 0, 0, 0}, total = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int s = slice; s < spans; s += slices) {
+      const quad_t c = *reinterpret_cast<const quad_t*>(counts + static_cast<std::size_t>(s) * digits + 4 * quad);
+      total += c;
+      before += s < static_cast<int>(blockIdx.x) ? c : quad_t{0, 0, 0, 0};
+    }
+    s_quad[slice * quads + quad] = before;  // [2][slices][quads]
+    s_quad[threads + slice * quads + quad] = total;
+  }
+  __syncthreads();
+  int before = 0, total = 0;
+  if (tid < 4 * quads)
+    for (int s = 0; s < slices; ++s) {
+      before += s_mem[4 * s * quads + tid];
+      total += s_mem[4 * threads + 4 * s * quads + tid];
+    }
+  const int base = detail::block_exclusive_sum(total, s_scan) + before;  // (its barriers end the use of s_mem)
+
+  // the workgroup's span, a sixteenth of it (a multiple of 64 items: span is a multiple of 1 024) per wavefront
+  int* const s_count = s_mem;  // [waves][digits]
   int* const mine = s_count + w * digits;
   for (int i = tid; i < waves * digits; i += threads) s_count[i] = 0;
   __syncthreads();
-
-  // the workgroup's span, a sixteenth of it (a multiple of 64 items: span is a multiple of 1 024) per wavefront
-  const int begin = blockIdx.x * span;
+  const int begin = static_cast<int>(blockIdx.x) * span;
   const int size = n - begin < span ? n - begin : span;
   const int part = span / waves;
   const int wave_begin = w * part < size ? w * part : size;
@@ -287,16 +280,7 @@ place_digits(const int n, const id_t* __restrict__ raw, const item_t* __restrict
     const unsigned int key = FIRST ? map(raw[begin + i]) : items[begin + i].key;
     atomicAdd(&mine[(key >> shift) & (digits - 1)], 1);
   }
-  int before = 0, total = 0;  // items of digit `tid` in the spans before this one / in all
-  if (tid < digits) {
-#pragma unroll 8
-    for (int s = 0; s < spans; ++s) {
-      const int c = counts[s * digits + tid];
-      total += c;
-      before += s < static_cast<int>(blockIdx.x) ? c : 0;
-    }
-  }
-  const int base = detail::block_exclusive_sum(total, s_scan) + before;  // (its barriers also order the counts above)
+  __syncthreads();
   detail::places(s_count, digits, base);
   __syncthreads();
   for (int i = wave_begin; i < wave_end; i += wave::size) {
@@ -321,35 +305,28 @@ template <typename id_t>
 int launch(hipStream_t stream, int n, const id_t* in, const key_map& map, int* ids, int* positions, void* workspace) {
   if (n == 0) return 0;
   const plan_t p = plan_for(n, map.rows);
-  if (p.spans == 1) {
-    if (n <= threads) launch_sort_block<1, id_t>(stream, n, in, map, p, ids, positions);
-    else if (n <= 4 * threads) launch_sort_block<4, id_t>(stream, n, in, map, p, ids, positions);
-    else launch_sort_block<8, id_t>(stream, n, in, map, p, ids, positions);
+  if (p.passes == 0) {
+    rank<id_t><<<(n + rank_group - 1) / rank_group, threads, 0, stream>>>(n, in, map, ids, positions);
     return static_cast<int>(hipGetLastError());
   }
-  const std::size_t stride = (static_cast<std::size_t>(n) * sizeof(item_t) + 255) & ~static_cast<std::size_t>(255);
   char* const at = static_cast<char*>(workspace);
   const int buffers = p.passes > 2 ? 2 : p.passes - 1;
-  item_t* const half[2] = {reinterpret_cast<item_t*>(at), reinterpret_cast<item_t*>(at + (buffers > 1 ? stride : 0))};
-  int* const counts = reinterpret_cast<int*>(at + stride * static_cast<std::size_t>(buffers));
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int shift = pass * p.bits;
-    const item_t* const from = half[(pass + 1) & 1];
-    item_t* const to = half[pass & 1];
-    const bool last = pass == p.passes - 1;
-    if (pass == 0) {
-      count_digits<true, id_t><<<p.spans, threads, 0, stream>>>(n, in, nullptr, map, shift, p.bits, p.span, counts);
-      if (last)
-        place_digits<true, true, id_t><<<p.spans, threads, 0, stream>>>(n, in, nullptr, map, shift, p.bits, p.span, p.spans, counts, nullptr, ids, positions);
-      else
-        place_digits<true, false, id_t><<<p.spans, threads, 0, stream>>>(n, in, nullptr, map, shift, p.bits, p.span, p.spans, counts, to, nullptr, nullptr);
-    } else {
-      count_digits<false, id_t><<<p.spans, threads, 0, stream>>>(n, nullptr, from, map, shift, p.bits, p.span, counts);
-      if (last)
-        place_digits<false, true, id_t><<<p.spans, threads, 0, stream>>>(n, nullptr, from, map, shift, p.bits, p.span, p.spans, counts, nullptr, ids, positions);
-      else
-        place_digits<false, false, id_t><<<p.spans, threads, 0, stream>>>(n, nullptr, from, map, shift, p.bits, p.span, p.spans, counts, to, nullptr, nullptr);
-    }
+  item_t* const half[2] = {reinterpret_cast<item_t*>(at), reinterpret_cast<item_t*>(at + (buffers > 1 ? item_bytes(n) : 0))};
+  int* const counts = reinterpret_cast<int*>(at + item_bytes(n) * static_cast<std::size_t>(buffers));
+  const auto pass = [&](auto first_tag, auto last_tag, int index) {
+    constexpr bool FIRST = decltype(first_tag)::value, LAST = decltype(last_tag)::value;
+    const int shift = index * p.bits;
+    const item_t* const from = FIRST ? nullptr : half[(index + 1) & 1];
+    count_digits<FIRST, id_t><<<p.spans, threads, 0, stream>>>(n, in, from, map, shift, p.bits, p.span, counts);
+    place_digits<FIRST, LAST, id_t><<<p.spans, threads, 0, stream>>>(n, in, from, map, shift, p.bits, p.span, p.spans, counts, half[index & 1], ids,
+                                                                    positions);
+  };
+  for (int i = 0; i < p.passes; ++i) {
+    const bool last = i == p.passes - 1;
+    if (i == 0 && last) pass(std::true_type{}, std::true_type{}, i);
+    else if (i == 0) pass(std::true_type{}, std::false_type{}, i);
+    else if (last) pass(std::false_type{}, std::true_type{}, i);
+    else pass(std::false_type{}, std::false_type{}, i);
   }
   return static_cast<int>(hipGetLastError());
 }
