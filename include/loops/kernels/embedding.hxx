@@ -32,7 +32,7 @@ constexpr int lookup_threads = 256;
  * written twice, with the same values): any width and alignment moves in 16-byte accesses.  Packets of all rows are numbered through
  * and each thread takes U of them, a workgroup's width apart: consecutive lanes touch consecutive packets whatever the width.
  */
-template <int V, int U, typename type_t, typename id_t>
+template <int V, int U, bool STREAM, typename type_t, typename id_t>
 __global__ void __launch_bounds__(lookup_threads)
 lookup(const type_t* __restrict__ table, const std::size_t table_pitch, const id_t* __restrict__ ids, const int tokens, const int packets,
        const int dim, const group_ids::key_map map, const float scale, type_t* __restrict__ out, const std::size_t out_pitch) {
@@ -70,7 +70,7 @@ lookup(const type_t* __restrict__ table, const std::size_t table_pitch, const id
       float v[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = inside ? static_cast<float>(packet[u][k]) * scale : 0.0f;
-      elements::store<V>(out + token[u] * out_pitch + column[u], v);
+      elements::store<V, STREAM>(out + token[u] * out_pitch + column[u], v);
     }
   }
 }
@@ -80,28 +80,32 @@ int launch_lookup(hipStream_t stream, const type_t* table, std::size_t table_pit
                   const group_ids::key_map& map, float scale, type_t* out, std::size_t out_pitch) {
   if (tokens == 0 || dim == 0) return 0;
   constexpr int V = elements::per_access<type_t>;
-  const auto run = [&](auto v_tag, auto u_tag) {
+  const auto run = [&](auto v_tag, auto u_tag, auto stream_tag) {
     constexpr int W = decltype(v_tag)::value, U = decltype(u_tag)::value;
     const int packets = (dim + W - 1) / W;
     const unsigned long long all = static_cast<unsigned long long>(tokens) * packets;
     const unsigned long long grid = (all + lookup_threads * U - 1) / (lookup_threads * U);
-    lookup<W, U, type_t, id_t><<<static_cast<unsigned int>(grid), lookup_threads, 0, stream>>>(table, table_pitch, ids, tokens, packets, dim, map,
-                                                                                               scale, out, out_pitch);
+    if (grid * lookup_threads >= (1ull << 32)) return static_cast<int>(hipErrorInvalidValue);
+    lookup<W, U, decltype(stream_tag)::value, type_t, id_t><<<static_cast<unsigned int>(grid), lookup_threads, 0, stream>>>(
+        table, table_pitch, ids, tokens, packets, dim, map, scale, out, out_pitch);
+    return static_cast<int>(hipGetLastError());
   };
+  using one = std::integral_constant<int, 1>;
+  using width = std::integral_constant<int, V>;
+  const bool whole_lines = (reinterpret_cast<std::uintptr_t>(out) | (out_pitch * sizeof(type_t)) | (dim * sizeof(type_t))) % 128 == 0;
   const bool many = static_cast<unsigned long long>(tokens) * dim >= 512ull * lookup_threads * 4 * V;
-  if (dim < V) run(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-  else if (many) run(std::integral_constant<int, V>{}, std::integral_constant<int, 4>{});
-  else run(std::integral_constant<int, V>{}, std::integral_constant<int, 1>{});
-  return static_cast<int>(hipGetLastError());
+  if (dim < V) return run(one{}, one{}, std::false_type{});
+  if (!many) return run(width{}, one{}, std::false_type{});
+  return whole_lines ? run(width{}, std::integral_constant<int, 4>{}, std::true_type{}) : run(width{}, std::integral_constant<int, 4>{}, std::false_type{});
 }
 
 // ---- gradient -----------------------------------------------------------------------------------------------------------------
 constexpr int gradient_threads = 256;
 constexpr int gradient_waves = gradient_threads / wave::size;
 
-/// Columns a wavefront covers.
-template <typename type_t>
-constexpr int slab = wave::size * elements::per_access<type_t>;
+/// Columns per lane: one 16-byte access of the wider of the two types, so that every store of a wavefront covers whole lines.
+template <typename type_t, typename out_t>
+constexpr int lane_width = elements::per_access<type_t> < elements::per_access<out_t> ? elements::per_access<type_t> : elements::per_access<out_t>;
 
 struct gradient_plan {
   int slabs;  ///< column slabs
@@ -114,12 +118,11 @@ struct gradient_plan {
  * load), or the tokens alone do (adding: rows without a token are not touched).  Equal tiles of that list, one wavefront per (tile,
  * slab of columns); a row of a hundred thousand tokens and a hundred thousand empty rows are the same work per wavefront.
  */
-template <typename type_t>
-gradient_plan gradient_plan_for(int tokens, int rows, int dim, bool add) {
+inline gradient_plan gradient_plan_for(int width, int tokens, int rows, int dim, bool add) {
   gradient_plan p;
-  p.slabs = (dim + slab<type_t> - 1) / slab<type_t>;
+  p.slabs = (dim + wave::size * width - 1) / (wave::size * width);
   const long long total = static_cast<long long>(tokens) + (add ? 0 : rows);
-  long long items = (total * p.slabs + 8191) / 8192;
+  long long items = (total * p.slabs + 16383) / 16384;
   items = items < 8 ? 8 : items;
   p.items = static_cast<int>(items);
   p.tiles = static_cast<int>((total + items - 1) / items);
@@ -133,9 +136,14 @@ struct tile_record {
   int tail_row;
 };
 
-/// Workspace: records[tiles], head[tiles][dim], tail[tiles][dim] (float).
+constexpr int small_tokens = 1024;  ///< most tokens of gradient_add_small
+
+/// Workspace: records[tiles], heads[tiles][dim], tails[tiles][dim] (float).
 inline std::size_t gradient_records_bytes(int tiles) { return (static_cast<std::size_t>(tiles) * sizeof(tile_record) + 255) & ~static_cast<std::size_t>(255); }
-inline std::size_t gradient_workspace_bytes(const gradient_plan& p, int dim) {
+template <typename type_t, typename out_t>
+std::size_t gradient_workspace_bytes(int tokens, int rows, int dim, bool add) {
+  if (dim == 0 || rows == 0 || (add && tokens <= small_tokens)) return 0;
+  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, rows, dim, add);
   return gradient_records_bytes(p.tiles) + 2 * static_cast<std::size_t>(p.tiles) * dim * sizeof(float);
 }
 
@@ -158,106 +166,107 @@ __device__ __forceinline__ int tokens_before(const int* __restrict__ keys, int t
   return lo;
 }
 
+/// A row of fewer tokens than this belongs to the tile of its first token; longer ones are cut at the tiles' ends and joined.
+constexpr int whole_row = wave::size;
+
+/// The columns of a lane in slab `part`; the last packet of a row is shifted back to end with it and keeps its own columns only.
+template <int V>
+struct lane_columns {
+  int at;
+  int skip;  ///< elements of the packet before the lane's own (V: none is the lane's)
+  bool whole;
+  __device__ __forceinline__ lane_columns(int part, int dim) {
+    const int own = (part * wave::size + wave::lane()) * V;
+    whole = own + V <= dim;
+    const bool active = own < dim;
+    at = whole ? own : active ? dim - V : 0;
+    skip = active ? own - at : V;
+  }
+  template <bool STREAM = false, typename T>
+  __device__ __forceinline__ void store(T* __restrict__ row, const float (&v)[V]) const {
+    if (whole) {
+      elements::store<V, STREAM>(row + at, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (k >= skip) row[at + k] = static_cast<T>(v[k]);
+    }
+  }
+};
+
+/// How many of the 64 tokens from `at` on (before it, for before = true) have this key.
+template <bool BEFORE>
+__device__ __forceinline__ int same_key(const int* __restrict__ keys, int tokens, int at, int key) {
+  const int j = BEFORE ? at - 1 - wave::lane() : at + wave::lane();
+  return __popcll(__ballot(j >= 0 && j < tokens && keys[j < 0 ? 0 : j < tokens ? j : tokens - 1] == key));
+}
+
+/// A position that group_ids did not write stays inside the array.
+__device__ __forceinline__ int bounded(int position, int tokens) {
+  return static_cast<unsigned int>(position) < static_cast<unsigned int>(tokens) ? position : 0;
+}
+
 /**
- * @tparam ADD  false: every row of grad is written (rows without tokens with zeros), true: rows with tokens are added to.
- * One wavefront per (tile, slab).  U gradient rows are in flight; ids and positions are wavefront-uniform (scalar loads).
+ * Every row of grad is written, rows without tokens with zeros.  One wavefront per (tile, slab); 64 tokens' keys and positions are loaded
+ * at a time, one per lane, and become scalars as the wavefront walks over them with U gradient rows in flight.
  */
-template <int V, int U, bool ADD, typename type_t, typename out_t>
+template <int V, int U, bool STREAM, typename type_t, typename out_t>
 __global__ void __launch_bounds__(gradient_threads)
-gradient(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows, const type_t* __restrict__ from,
-         const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad, const std::size_t grad_pitch, const int tiles,
-         const int items, const int slabs, tile_record* __restrict__ records, float* __restrict__ heads, float* __restrict__ tails) {
+gradient_overwrite(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows,
+                   const type_t* __restrict__ from, const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad,
+                   const std::size_t grad_pitch, const int tiles, const int items, const int slabs, tile_record* __restrict__ records,
+                   float* __restrict__ heads, float* __restrict__ tails) {
   const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * gradient_waves + static_cast<int>(threadIdx.x) / wave::size);
   const int tile = unit / slabs;
   if (tile >= tiles) return;
   const int part = unit - tile * slabs;
-  // the lane's columns; the last packet of a row is shifted back to end with it and stores its own columns only
-  const int own = (part * wave::size + wave::lane()) * V;
-  const bool active = own < dim;
-  const bool whole = own + V <= dim;
-  const int column = whole ? own : active ? dim - V : 0;
-  const int skip = active ? own - column : V;
-
-  const long long total = static_cast<long long>(tokens) + (ADD ? 0 : rows);
+  const lane_columns<V> cols(part, dim);
+  const long long total = static_cast<long long>(tokens) + rows;
   const long long d0 = static_cast<long long>(tile) * items;
   const long long d1 = d0 + items < total ? d0 + items : total;
-  int y = ADD ? static_cast<int>(d0) : __builtin_amdgcn_readfirstlane(tokens_before(keys, tokens, d0));
-  const int before = y > 0 ? keys[y - 1] : -1;  // the row of the token before the tile
-  int row = ADD ? (y < tokens ? keys[y] : rows) : static_cast<int>(d0 - y);
-  bool open = before == row && row < rows;  // the row was begun by an earlier tile
-  bool some = false;                        // tokens of this tile in the row
+  int y = __builtin_amdgcn_readfirstlane(tokens_before(keys, tokens, d0));
+  int row = static_cast<int>(d0 - y);
+  bool open = false;  // the row was begun by an earlier tile, and is cut here
+  if (y > 0 && row < rows && keys[y - 1] == row) {
+    const int behind = same_key<false>(keys, tokens, y, row);
+    open = same_key<true>(keys, tokens, y, row) + behind >= whole_row;
+    if (!open) {  // all of it, end included, is the earlier tile's
+      y += behind;
+      ++row;
+    }
+  }
+  int begun = y;      // the row's first token here
   int head_row = -1;
-
-  const type_t* __restrict__ const base = from + column;
   float acc[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.0f;
 
-  const auto put_partial = [&](float* __restrict__ to) {
-    if (active) {
-      float* const at = to + static_cast<std::size_t>(tile) * dim;
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (k >= skip) at[column + k] = acc[k];
-    }
-  };
   const auto finish = [&]() {  // the row's end
     if (open) {
       head_row = row;
-      put_partial(heads);
+      cols.store(heads + static_cast<std::size_t>(tile) * dim, acc);
       open = false;
-    } else if (!ADD || some) {
-      out_t* const at = grad + static_cast<std::size_t>(row) * grad_pitch + column;
+    } else {
       float v[V];
-      if (whole) {
-        if constexpr (ADD) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = __builtin_fmaf(scale, acc[k], static_cast<float>(at[k]));
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = scale * acc[k];
-        }
-        elements::store<V>(at, v);
-      } else if (active) {
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (k >= skip) at[k] = static_cast<out_t>(ADD ? __builtin_fmaf(scale, acc[k], static_cast<float>(at[k])) : scale * acc[k]);
-      }
+      for (int k = 0; k < V; ++k) v[k] = scale * acc[k];
+      cols.template store<STREAM>(grad + static_cast<std::size_t>(row) * grad_pitch, v);
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-    some = false;
+    ++row;
   };
-  const auto clear = [&]() {  // a row without tokens
-    out_t* const at = grad + static_cast<std::size_t>(row) * grad_pitch + column;
+  const auto clear_below = [&](int to) {  // rows without tokens
     const float zero[V] = {};
-    if (whole) {
-      elements::store<V>(at, zero);
-    } else if (active) {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (k >= skip) at[k] = static_cast<out_t>(0.0f);
-    }
+    for (; row < to; ++row) cols.template store<STREAM>(grad + static_cast<std::size_t>(row) * grad_pitch, zero);
   };
-
-  // 64 tokens' keys and positions at a time, a token per lane; the tile's are a prefix of them
-  for (;;) {
-    const int j = y + wave::lane();
-    int key = rows, position = 0;
-    if (j < tokens) {
-      key = keys[j];
-      position = positions[j];
-    }
-    // (a position that group_ids did not write stays inside the array)
-    if (static_cast<unsigned int>(position) >= static_cast<unsigned int>(tokens)) position = 0;
-    const bool mine = key < rows && static_cast<long long>(j) + (ADD ? 0 : key) < d1;
-    const int count = __popcll(__ballot(mine));
+  const auto consume = [&](int key, int position, int count) {  // tokens y .. y + count, a lane each
     for (int i = 0; i < count; i += U) {
       elements::packet_t<type_t, V> packet[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = i + u < count ? i + u : count - 1;
-        packet[u] = elements::load<V>(base + static_cast<std::size_t>(__builtin_amdgcn_readlane(position, at)) * from_pitch);
+        packet[u] = elements::load<V>(from + static_cast<std::size_t>(__builtin_amdgcn_readlane(position, at)) * from_pitch + cols.at);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -265,47 +274,241 @@ gradient(const int* __restrict__ keys, const int* __restrict__ positions, const 
           const int k = __builtin_amdgcn_readlane(key, i + u);
           if (row < k) {
             finish();
-            if constexpr (ADD) row = k;
-            else
-              for (++row; row < k; ++row) clear();
+            clear_below(k);
+            begun = y + i + u;
           }
-          some = true;
 #pragma unroll
           for (int c = 0; c < V; ++c) acc[c] += static_cast<float>(packet[u][c]);
         }
       }
     }
     y += count;
-    if (count < wave::size) break;
-  }
-  // the rows that end in what is left of the tile
-  bool unfinished;
-  if constexpr (ADD) {
-    unfinished = some && y < tokens && keys[y] == row;
-    if (some && !unfinished) finish();
-  } else {
-    const int row1 = d1 - y < rows ? static_cast<int>(d1 - y) : rows;  // (tokens without a row lie behind all of them)
-    if (row < row1) {
-      finish();
-      for (++row; row < row1; ++row) clear();
+  };
+
+  int next_key = rows;  // of the token behind the tile's
+  for (;;) {
+    const int j = y + wave::lane();
+    int key = rows, position = 0;
+    if (j < tokens) {
+      key = keys[j];
+      position = bounded(positions[j], tokens);
     }
-    unfinished = some || open;
+    const bool mine = key < rows && static_cast<long long>(j) + key < d1;  // (a prefix of the lanes)
+    const int count = __popcll(__ballot(mine));
+    consume(key, position, count);
+    if (count < wave::size) {
+      next_key = __builtin_amdgcn_readlane(key, count);
+      break;
+    }
   }
-  if (unfinished) put_partial(tails);
+  // the rows that end in what is left of the tile (tokens without a row lie behind all of them)
+  const int row1 = d1 - y < rows ? static_cast<int>(d1 - y) : rows;
+  if (row < row1) {
+    finish();
+    clear_below(row1);
+    begun = y;
+  }
+  bool unfinished = open || y > begun;
+  if (unfinished && !open) {
+    const int behind = next_key == row ? same_key<false>(keys, tokens, y, row) : 0;
+    if (y - begun + behind < whole_row) {  // a short row is finished here
+      const int j = y + wave::lane();
+      consume(row, j < tokens ? bounded(positions[j], tokens) : 0, behind);
+      finish();
+      unfinished = false;
+    }
+  }
+  if (unfinished) cols.store(tails + static_cast<std::size_t>(tile) * dim, acc);
   if (part == 0 && wave::lane() == 0) records[tile] = tile_record{head_row, unfinished ? row : -1};
 }
 
 /**
+ * Rows with tokens are added to.  Tiles of `items` tokens; otherwise as above.  What a row held is read together with the gradient
+ * row of its last token, so that the two latencies are one.
+ */
+template <int V, int U, typename type_t, typename out_t>
+__global__ void __launch_bounds__(gradient_threads)
+gradient_add(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows, const type_t* __restrict__ from,
+             const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad, const std::size_t grad_pitch,
+             const int tiles, const int items, const int slabs, tile_record* __restrict__ records, float* __restrict__ heads,
+             float* __restrict__ tails) {
+  const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * gradient_waves + static_cast<int>(threadIdx.x) / wave::size);
+  const int tile = unit / slabs;
+  if (tile >= tiles) return;
+  const int part = unit - tile * slabs;
+  const lane_columns<V> cols(part, dim);
+  const long long d0 = static_cast<long long>(tile) * items;
+  int y = static_cast<int>(d0);
+  const int end = d0 + items < tokens ? static_cast<int>(d0 + items) : tokens;
+  int row = keys[y];
+  bool open = false;  // the row was begun by an earlier tile, and is cut here
+  if (y > 0 && row < rows && keys[y - 1] == row) {
+    const int behind = same_key<false>(keys, tokens, y, row);
+    open = same_key<true>(keys, tokens, y, row) + behind >= whole_row;
+    if (!open) y += behind;
+  }
+  int begun = y;  // the row's first token here
+  int head_row = -1;
+  float acc[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+
+  const auto consume = [&](int key, int position, unsigned long long last, int count) {  // tokens y .. y + count; last: bits of the rows' ends
+    for (int i = 0; i < count; i += U) {
+      elements::packet_t<type_t, V> packet[U];
+      elements::packet_t<out_t, V> old[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = i + u < count ? i + u : count - 1;
+        packet[u] = elements::load<V>(from + static_cast<std::size_t>(__builtin_amdgcn_readlane(position, at)) * from_pitch + cols.at);
+        if ((last >> at) & 1ull) old[u] = elements::load<V>(grad + static_cast<std::size_t>(__builtin_amdgcn_readlane(key, at)) * grad_pitch + cols.at);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u < count) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[c] += static_cast<float>(packet[u][c]);
+          if ((last >> (i + u)) & 1ull) {
+            const int k = __builtin_amdgcn_readlane(key, i + u);
+            if (open) {
+              head_row = k;
+              cols.store(heads + static_cast<std::size_t>(tile) * dim, acc);
+              open = false;
+            } else {
+              float v[V];
+#pragma unroll
+              for (int c = 0; c < V; ++c) v[c] = __builtin_fmaf(scale, acc[c], static_cast<float>(old[u][c]));
+              cols.store(grad + static_cast<std::size_t>(k) * grad_pitch, v);
+            }
+#pragma unroll
+            for (int c = 0; c < V; ++c) acc[c] = 0.0f;
+            begun = y + i + u + 1;
+          }
+        }
+      }
+    }
+    y += count;
+  };
+
+  while (y < end) {
+    const int j = y + wave::lane();
+    int key = rows, next = rows, position = 0;
+    if (j < tokens) {
+      key = keys[j];
+      position = bounded(positions[j], tokens);
+      if (j + 1 < tokens) next = keys[j + 1];
+    }
+    const int count = __popcll(__ballot(key < rows && j < end));
+    if (count == 0) break;
+    const unsigned long long last = __ballot(key != next);
+    row = __builtin_amdgcn_readlane(key, count - 1);
+    consume(key, position, last, count);
+    if (count < wave::size) break;
+  }
+  bool unfinished = y > begun;
+  if (unfinished && !open) {
+    const int behind = same_key<false>(keys, tokens, y, row);  // (at least one: the row's last token was not the tile's)
+    if (y - begun + behind < whole_row) {
+      const int j = y + wave::lane();
+      consume(row, j < tokens ? bounded(positions[j], tokens) : 0, 1ull << (behind - 1), behind);
+      unfinished = false;
+    }
+  }
+  if (unfinished) cols.store(tails + static_cast<std::size_t>(tile) * dim, acc);
+  if (part == 0 && wave::lane() == 0) records[tile] = tile_record{head_row, unfinished ? row : -1};
+}
+
+constexpr int small_threads = 1024;
+constexpr int small_waves = small_threads / wave::size;
+static_assert(small_tokens <= small_waves * wave::size, "a token per lane");
+
+/**
+ * gradient_add for few tokens, in one launch: a workgroup adds all tokens of 64 columns, a sixteenth of them per wavefront, and rows
+ * that several wavefronts hold are joined in LDS.  One column per lane: a row of the gradient is spread over as many CUs as there are
+ * slabs (1 024 columns: 16), which few tokens leave idle otherwise.
+ */
+template <int U, typename type_t, typename out_t>
+__global__ void __launch_bounds__(small_threads)
+gradient_add_small(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows,
+                   const type_t* __restrict__ from, const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad,
+                   const std::size_t grad_pitch) {
+  __shared__ float s_tail[small_waves][wave::size];
+  __shared__ int s_tail_row[small_waves];
+  const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / wave::size);
+  const int lane = wave::lane();
+  const int column = static_cast<int>(blockIdx.x) * wave::size + lane;
+  const bool active = column < dim;
+  const int at = active ? column : 0;
+  const int items = (tokens + small_waves - 1) / small_waves;  // at most 64: a token per lane
+  const int begin = w * items < tokens ? w * items : tokens;
+  const int end = begin + items < tokens ? begin + items : tokens;
+  const int j = begin + lane;
+  int key = rows, next = rows, position = 0;
+  if (j < end) {
+    key = keys[j];
+    position = bounded(positions[j], tokens);
+    if (j + 1 < tokens) next = keys[j + 1];
+  }
+  const int count = __popcll(__ballot(key < rows));
+  const unsigned long long last = __ballot(key != next);
+  bool open = count > 0 && begin > 0 && keys[begin - 1] == __builtin_amdgcn_readfirstlane(key);
+  int head_row = -1;
+  float acc = 0.0f, head = 0.0f, head_old = 0.0f;
+  for (int i = 0; i < count; i += U) {
+    type_t value[U];
+    out_t old[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = i + u < count ? i + u : count - 1;
+      value[u] = from[static_cast<std::size_t>(__builtin_amdgcn_readlane(position, t)) * from_pitch + at];
+      old[u] = grad[static_cast<std::size_t>(__builtin_amdgcn_readlane(key, t)) * grad_pitch + at];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u < count) {
+        acc += static_cast<float>(value[u]);
+        if ((last >> (i + u)) & 1ull) {
+          const int row = __builtin_amdgcn_readlane(key, i + u);
+          if (open) {
+            head_row = row;
+            head = acc;
+            head_old = static_cast<float>(old[u]);
+            open = false;
+          } else if (active) {
+            grad[static_cast<std::size_t>(row) * grad_pitch + at] = static_cast<out_t>(__builtin_fmaf(scale, acc, static_cast<float>(old[u])));
+          }
+          acc = 0.0f;
+        }
+      }
+    }
+  }
+  const bool unfinished = count > 0 && !((last >> (count - 1)) & 1ull);
+  s_tail[w][lane] = acc;
+  if (lane == 0) s_tail_row[w] = unfinished ? __builtin_amdgcn_readlane(key, count > 0 ? count - 1 : 0) : -1;
+  __syncthreads();
+  if (head_row >= 0 && active) {
+    int first = w;
+    while (first > 0 && s_tail_row[first - 1] == head_row) --first;
+    float sum = 0.0f;
+    for (int i = first; i < w; ++i) sum += s_tail[i][lane];
+    grad[static_cast<std::size_t>(head_row) * grad_pitch + at] = static_cast<out_t>(__builtin_fmaf(scale, sum + head, head_old));
+  }
+}
+
+constexpr int join_threads = 512;
+constexpr int join_waves = join_threads / wave::size;
+
+/**
  * The rows that more than one tile holds: sum of the tails of the tiles before, in a fixed order, and the finishing tile's head.
- * A workgroup covers 256 columns and walks over every gridDim.y-th run of 64 tiles; its four wavefronts share a row's tails out.
+ * A workgroup covers 256 columns and every gridDim.y-th tile; its wavefronts share a row's tails out.
  */
 template <bool ADD, typename out_t>
-__global__ void __launch_bounds__(gradient_threads)
+__global__ void __launch_bounds__(join_threads)
 join(const tile_record* __restrict__ records, const float* __restrict__ heads, const float* __restrict__ tails, const int tiles, const int dim,
      const float scale, out_t* __restrict__ grad, const std::size_t grad_pitch) {
   constexpr int C = 4;  // columns per lane
   constexpr int U = 8;
-  __shared__ float s_sum[gradient_waves][C][wave::size];
+  __shared__ float s_sum[join_waves][C][wave::size];
   const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / wave::size);
   const int lane = wave::lane();
   const int own = (static_cast<int>(blockIdx.x) * wave::size + lane) * C;
@@ -321,34 +524,32 @@ join(const tile_record* __restrict__ records, const float* __restrict__ heads, c
       for (int c = 0; c < C; ++c) v[c] = c < mine ? at[c] : 0.0f;
     }
   };
-  for (int t0 = static_cast<int>(blockIdx.y) * wave::size; t0 < tiles; t0 += static_cast<int>(gridDim.y) * wave::size) {
-    const int head = t0 + lane < tiles ? records[t0 + lane].head_row : -1;
+  const int stride = static_cast<int>(gridDim.y);
+  for (int t0 = static_cast<int>(blockIdx.y); t0 < tiles; t0 += stride * wave::size) {
+    const long long t = static_cast<long long>(t0) + static_cast<long long>(lane) * stride;
+    const int head = t < tiles ? records[t].head_row : -1;
     unsigned long long todo = __ballot(head >= 0);
     while (todo) {
       const int at = __builtin_ctzll(todo);
       todo &= todo - 1;
-      const int tile = t0 + at;
+      const int tile = t0 + at * stride;
       const int row = __builtin_amdgcn_readlane(head, at);
       int run = 0;  // tiles before this one that hold a part of the row
       for (;;) {
-        const int t = tile - 1 - run - lane;
-        const unsigned long long part = __ballot(t >= 0 && records[t < 0 ? 0 : t].tail_row == row);
+        const int b = tile - 1 - run - lane;
+        const unsigned long long part = __ballot(b >= 0 && records[b < 0 ? 0 : b].tail_row == row);
         const int n = part == ~0ull ? wave::size : __builtin_ctzll(~part);
         run += n;
         if (n < wave::size) break;
       }
       float sum[C] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const int first = tile - run;
-      for (int t = first + w; t < tile; t += gradient_waves * U) {
+      for (int b = tile - run + w; b < tile; b += join_waves * U) {
         float v[U][C];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int from = t + u * gradient_waves;
-          read(tails, from < tile ? from : tile - 1, v[u]);
-        }
+        for (int u = 0; u < U; ++u) read(tails, b + u * join_waves < tile ? b + u * join_waves : tile - 1, v[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (t + u * gradient_waves < tile) {
+          if (b + u * join_waves < tile) {
 #pragma unroll
             for (int c = 0; c < C; ++c) sum[c] += v[u][c];
           }
@@ -364,7 +565,7 @@ join(const tile_record* __restrict__ records, const float* __restrict__ heads, c
         for (int c = 0; c < C; ++c) {
           float v = s_sum[0][c][lane];
 #pragma unroll
-          for (int i = 1; i < gradient_waves; ++i) v += s_sum[i][c][lane];
+          for (int i = 1; i < join_waves; ++i) v += s_sum[i][c][lane];
           v += last[c];
           if (c < mine) to[c] = static_cast<out_t>(ADD ? __builtin_fmaf(scale, v, static_cast<float>(to[c])) : scale * v);
         }
@@ -378,24 +579,39 @@ template <typename type_t, typename out_t>
 int launch_gradient(hipStream_t stream, const int* keys, const int* positions, int tokens, int rows, const type_t* from, std::size_t from_pitch,
                     int dim, float scale, bool add, out_t* grad, std::size_t grad_pitch, void* workspace) {
   if (rows == 0 || dim == 0 || (tokens == 0 && add)) return 0;
-  const gradient_plan p = gradient_plan_for<type_t>(tokens, rows, dim, add);
+  if (add && tokens <= small_tokens) {
+    gradient_add_small<16, type_t, out_t><<<(dim + wave::size - 1) / wave::size, small_threads, 0, stream>>>(keys, positions, tokens, rows, from,
+                                                                                                        from_pitch, dim, scale, grad, grad_pitch);
+    return static_cast<int>(hipGetLastError());
+  }
+  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, rows, dim, add);
   auto* const records = static_cast<tile_record*>(workspace);
   float* const heads = reinterpret_cast<float*>(static_cast<char*>(workspace) + gradient_records_bytes(p.tiles));
   float* const tails = heads + static_cast<std::size_t>(p.tiles) * dim;
   const unsigned int grid = (static_cast<unsigned int>(p.tiles) * p.slabs + gradient_waves - 1) / gradient_waves;
   const int column_groups = (dim + 255) / 256;
-  const int tile_groups = (p.tiles + wave::size - 1) / wave::size;
-  const int most = 1024 / column_groups > 1 ? 1024 / column_groups : 1;
-  const dim3 join_grid(column_groups, tile_groups < most ? tile_groups : most);
+  const int most = 2048 / column_groups > 1 ? 2048 / column_groups : 1;
+  const dim3 join_grid(column_groups, p.tiles < most ? p.tiles : most);
+  const bool whole_lines = (reinterpret_cast<std::uintptr_t>(grad) | (grad_pitch * sizeof(out_t)) | (dim * sizeof(out_t))) % 128 == 0;
   const auto run = [&](auto v_tag, auto add_tag) {
     constexpr int V = decltype(v_tag)::value;
     constexpr bool ADD = decltype(add_tag)::value;
-    gradient<V, 8, ADD, type_t, out_t><<<grid, gradient_threads, 0, stream>>>(keys, positions, tokens, rows, from, from_pitch, dim, scale, grad,
-                                                                             grad_pitch, p.tiles, p.items, p.slabs, records, heads, tails);
-    if (p.tiles > 1)
-      join<ADD, out_t><<<join_grid, gradient_threads, 0, stream>>>(records, heads, tails, p.tiles, dim, scale, grad, grad_pitch);
+    if constexpr (ADD) {
+      gradient_add<V, 4, type_t, out_t><<<grid, gradient_threads, 0, stream>>>(keys, positions, tokens, rows, from, from_pitch, dim, scale, grad,
+                                                                              grad_pitch, p.tiles, p.items, p.slabs, records, heads, tails);
+    } else {
+      constexpr int U = V * sizeof(type_t) > 8 ? 8 : 16;  // 8 to 16 KB of a wavefront's loads in flight
+      const auto overwrite = [&](auto stream_tag) {
+        gradient_overwrite<V, U, decltype(stream_tag)::value, type_t, out_t><<<grid, gradient_threads, 0, stream>>>(
+            keys, positions, tokens, rows, from, from_pitch, dim, scale, grad, grad_pitch, p.tiles, p.items, p.slabs, records, heads, tails);
+      };
+      if (whole_lines) overwrite(std::true_type{});
+      else overwrite(std::false_type{});
+    }
+    if (p.tiles > 1 && tokens >= whole_row)
+      join<ADD, out_t><<<join_grid, join_threads, 0, stream>>>(records, heads, tails, p.tiles, dim, scale, grad, grad_pitch);
   };
-  constexpr int V = elements::per_access<type_t>;
+  constexpr int V = lane_width<type_t, out_t>;
   if (dim < V) {
     if (add) run(std::integral_constant<int, 1>{}, std::true_type{});
     else run(std::integral_constant<int, 1>{}, std::false_type{});

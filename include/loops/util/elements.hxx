@@ -1,6 +1,6 @@
 /**
  * @file elements.hxx
- * @brief Elements of 16 and 32 bits (float, _Float16, __bf16) moved as packets of V consecutive values, with one access of up to 16
+ * @brief Elements of 16 and 32 bits (float, _Float16, __bf16) moved as packets of V consecutive values, in accesses of up to 16
  * bytes at ANY element alignment (gfx950 takes 16-byte accesses at addresses that are only aligned to the element), and converted
  * to float for the arithmetic between.  A store rounds each value once, to nearest even.
  */
@@ -30,7 +30,6 @@ using packet_t = typename detail::packet<T, V>::type;
 /// STREAM: the lines are not expected to be read again soon.
 template <int V, bool STREAM = false, typename T>
 __device__ __forceinline__ packet_t<T, V> load(const T* __restrict__ p) {
-  static_assert(V * sizeof(T) <= 16, "one access");
   const auto* at = reinterpret_cast<const typename detail::packet<T, V>::unaligned*>(p);
   if constexpr (STREAM) return __builtin_nontemporal_load(at);
   else return *at;
@@ -39,24 +38,12 @@ __device__ __forceinline__ packet_t<T, V> load(const T* __restrict__ p) {
 /// V floats to p, each rounded to T.
 template <int V, bool STREAM = false, typename T>
 __device__ __forceinline__ void store(T* __restrict__ p, const float (&in)[V]) {
-  if constexpr (V * sizeof(T) > 16) {  // float beside a 16-bit type: two accesses
-    constexpr int H = V / 2;
-    float lo[H], hi[H];
+  packet_t<T, V> v;
 #pragma unroll
-    for (int k = 0; k < H; ++k) {
-      lo[k] = in[k];
-      hi[k] = in[H + k];
-    }
-    store<H, STREAM>(p, lo);
-    store<H, STREAM>(p + H, hi);
-  } else {
-    packet_t<T, V> v;
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = static_cast<T>(in[k]);
-    auto* at = reinterpret_cast<typename detail::packet<T, V>::unaligned*>(p);
-    if constexpr (STREAM) __builtin_nontemporal_store(v, at);
-    else *at = v;
-  }
+  for (int k = 0; k < V; ++k) v[k] = static_cast<T>(in[k]);
+  auto* at = reinterpret_cast<typename detail::packet<T, V>::unaligned*>(p);
+  if constexpr (STREAM) __builtin_nontemporal_store(v, at);
+  else *at = v;
 }
 
 }  // namespace elements

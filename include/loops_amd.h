@@ -578,7 +578,8 @@ int loops_allgatherv_f64(void* comm, int rank, int world, double* y_full, const 
  * (include/loops/kernels/embedding.hxx, group_ids.hxx).
  * Values are float, half or bfloat16 (enum loops_value_type), ids are int or long long (enum loops_index_type); another number
  * returns LOOPS_E_CONFIG.  Matrices are row-major with unit column stride; a pitch is the distance of two rows in elements (>= the
- * row's width, LOOPS_E_BADARG otherwise), at any alignment of the element.  No output may overlap an input.
+ * row's width, LOOPS_E_BADARG otherwise), at any alignment of the element.  An output that overlaps an input (by the
+ * addresses between their first and last elements) is LOOPS_E_BADARG.
  * `first_id` (>= 0): the id of the table's row 0.  A token whose id is outside [first_id, first_id + rows) -- padding, or a row that
  * another rank's shard of the table holds -- has a zero row in the lookup and no part in the gradient; no id is an error.
  * Calls are asynchronous and may be captured; they keep nothing between calls: scratch memory is the caller's `workspace`
@@ -602,7 +603,7 @@ int loops_group_tokens(int index_type, int tokens, const void* token_ids, int ro
  * loops_group_tokens wrote them for these tokens and rows.  accumulate = 0: every row of `out` is written (zeros where there is no
  * token); otherwise the sums are added to what rows with tokens hold and the other rows are left as they are.  `out` has `grad_type`
  * or is float (LOOPS_E_CONFIG otherwise).  The order of summation is fixed: equal inputs give equal bits. */
-int loops_embedding_gradient_workspace(int grad_type, int tokens, int rows, int dim, int accumulate, size_t* bytes);
+int loops_embedding_gradient_workspace(int grad_type, int out_type, int tokens, int rows, int dim, int accumulate, size_t* bytes);
 int loops_embedding_gradient(int grad_type, int out_type, int tokens, const int* ids, const int* positions, int rows, int dim,
                              const void* grad, long long grad_pitch, float scale, int accumulate, void* out, long long out_pitch,
                              void* workspace, size_t workspace_bytes, void* stream);

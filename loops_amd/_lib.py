@@ -268,7 +268,7 @@ def lib() -> C.CDLL:
         L.loops_embedding_lookup.argtypes = [ci, ci, ci, ci, vp, cll, ci, vp, cll, cf, vp, cll, vp]
         L.loops_group_tokens_workspace.argtypes = [ci, ci, C.POINTER(size)]
         L.loops_group_tokens.argtypes = [ci, ci, vp, ci, cll, cll, vp, vp, vp, size, vp]
-        L.loops_embedding_gradient_workspace.argtypes = [ci, ci, ci, ci, ci, C.POINTER(size)]
+        L.loops_embedding_gradient_workspace.argtypes = [ci, ci, ci, ci, ci, ci, C.POINTER(size)]
         L.loops_embedding_gradient.argtypes = [ci, ci, ci, vp, vp, ci, ci, vp, cll, cf, ci, vp, cll, vp, size, vp]
         L.loops_expert_counts_workspace.argtypes = [ci, ci, ci, C.POINTER(size)]
         L.loops_expert_counts.argtypes = [ci, ci, ci, vp, vp, ci, vp, vp, size, vp]

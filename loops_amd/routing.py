@@ -7,7 +7,8 @@ With p = softmax(logits), c the counts, n the number of tokens whose mask holds 
 
 The order in which experts take their tokens is ``embedding.group_tokens(chosen, experts)``.  Logits are float32, float16 or bfloat16,
 expert indices int32 or int64 (one outside [0, experts) is not counted).  Calls are asynchronous on the current stream of the tensors'
-device and may be captured into a graph; there is no CPU path.
+device and may be captured into a graph; there is no CPU path.  Arguments of a wrong type raise TypeError, of a wrong shape or layout
+ValueError; what the library itself refuses (an output that overlaps an input, sizes beyond its range) LoopsError.
 """
 from __future__ import annotations
 
@@ -15,7 +16,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .embedding import index_type, launch, overlap, pitch_of, require, same_device, value_type, workspace
+from .embedding import index_type, launch, pitch_of, same_device, value_type, workspace
 
 
 def _mask(mask: Optional[torch.Tensor], tokens: int):
@@ -23,7 +24,8 @@ def _mask(mask: Optional[torch.Tensor], tokens: int):
         return None
     if mask.dtype not in (torch.bool, torch.uint8):
         raise TypeError("mask must be bool or uint8")
-    require(mask.is_contiguous() and mask.numel() == tokens, "mask must be contiguous with an element for each token")
+    if not mask.is_contiguous() or mask.numel() != tokens:
+        raise ValueError("mask must be contiguous with an element for each token")
     return mask.data_ptr()
 
 
@@ -31,7 +33,8 @@ def expert_counts(chosen: torch.Tensor, experts: int, mask: Optional[torch.Tenso
     """int32 [experts]: how often each expert stands in ``chosen`` ([tokens, choices] or [tokens], contiguous), in the rows whose
     ``mask`` holds."""
     index = index_type(chosen, "chosen")
-    require(chosen.dim() in (1, 2) and chosen.is_contiguous(), "chosen must be [tokens, choices], contiguous")
+    if chosen.dim() not in (1, 2) or not chosen.is_contiguous():
+        raise ValueError("chosen must be [tokens, choices], contiguous")
     tokens = chosen.shape[0]
     choices = chosen.shape[1] if chosen.dim() == 2 else 1
     device = same_device(chosen, mask)
@@ -58,17 +61,19 @@ def balance_loss(logits: torch.Tensor, chosen: torch.Tensor, coefficient: float 
     value, index = value_type(logits, "logits"), index_type(chosen, "chosen")
     pitch = pitch_of(logits, "logits")
     tokens, experts = logits.shape
-    require(chosen.dim() == 2 and chosen.shape[0] == tokens and chosen.is_contiguous(), "chosen must be [tokens, choices], contiguous")
+    if chosen.dim() != 2 or chosen.shape[0] != tokens or not chosen.is_contiguous():
+        raise ValueError("chosen must be [tokens, choices], contiguous")
     choices = chosen.shape[1]
     device = same_device(logits, chosen, mask)
     masked = _mask(mask, tokens)
     _keep, ws, size = workspace(device, "loops_balance_loss_workspace", tokens, experts)
-    whole = torch.empty(experts + 1, dtype=torch.int32, device=device)
-    real = torch.empty(experts + 1, dtype=torch.float32, device=device)
-    at_whole, at_real = whole.data_ptr(), real.data_ptr()
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    counts = torch.empty(experts, dtype=torch.int32, device=device)
+    probability = torch.empty(experts, dtype=torch.float32, device=device)
+    counted = torch.empty((), dtype=torch.int32, device=device)
     launch(device, "loops_balance_loss", value, index, tokens, experts, choices, logits.data_ptr(), pitch, chosen.data_ptr(), masked, coefficient,
-           at_real + 4 * experts, at_whole, at_real, at_whole + 4 * experts, ws, size)
-    return BalanceLoss(real[experts], whole[:experts], real[:experts], whole[experts], choices, coefficient)
+           loss.data_ptr(), counts.data_ptr(), probability.data_ptr(), counted.data_ptr(), ws, size)
+    return BalanceLoss(loss, counts, probability, counted, choices, coefficient)
 
 
 def balance_loss_backward(logits: torch.Tensor, forward: BalanceLoss, mask: Optional[torch.Tensor] = None, grad_loss: Optional[torch.Tensor] = None,
@@ -78,21 +83,26 @@ def balance_loss_backward(logits: torch.Tensor, forward: BalanceLoss, mask: Opti
     value = value_type(logits, "logits")
     pitch = pitch_of(logits, "logits")
     tokens, experts = logits.shape
-    require(forward.counts.shape == (experts,), "forward was made of another number of experts")
+    if forward.counts.shape != (experts,):
+        raise ValueError("forward was made of another number of experts")
     device = same_device(logits, forward.counts, forward.tokens, mask, grad_loss, out)
     masked = _mask(mask, tokens)
     upstream = None
     if grad_loss is not None:
         if grad_loss.dtype is not torch.float32:
             raise TypeError("grad_loss must be float32")
-        require(grad_loss.numel() == 1, "grad_loss must be a scalar")
+        if grad_loss.numel() != 1:
+            raise ValueError("grad_loss must be a scalar")
         upstream = grad_loss.data_ptr()
     if out is None:
         out = torch.empty(tokens, experts, dtype=logits.dtype, device=device)
+        out_pitch = experts
     else:
-        require(out.dtype is logits.dtype and out.shape == logits.shape, "out must have the logits' shape and type")
-        require(not overlap(out, logits) and not overlap(out, forward.counts) and not overlap(out, forward.tokens) and
-                (mask is None or not overlap(out, mask)) and (grad_loss is None or not overlap(out, grad_loss)), "out must not overlap the inputs")
+        if out.dtype is not logits.dtype:
+            raise TypeError("out must have the logits' type")
+        if out.shape != logits.shape:
+            raise ValueError("out must have the logits' shape")
+        out_pitch = pitch_of(out, "out")
     launch(device, "loops_balance_loss_backward", value, tokens, experts, forward.choices, logits.data_ptr(), pitch, forward.counts.data_ptr(),
-           forward.tokens.data_ptr(), masked, forward.coefficient, upstream, out.data_ptr(), pitch_of(out, "out"))
+           forward.tokens.data_ptr(), masked, forward.coefficient, upstream, out.data_ptr(), out_pitch)
     return out
