@@ -34,8 +34,9 @@ constexpr int max_groups = 512;  ///< workgroups whose partial sums the finish k
 namespace detail {
 
 /// Which columns of a row a lane holds: K packets of V, packet k of lane l (of the G that share the row) is packet l + k G of the row.
-/// The row's last packet is shifted back to end with it; its first `skip` elements belong to the packet before.
-template <int V, int G, int K>
+/// FULL: the row is G K V columns.  Otherwise its last packet is shifted back to end with it, and the first `skip` elements of that belong
+/// to the packet before.
+template <bool FULL, int V, int G, int K>
 struct columns {
   int at[K];
   int skip[K];  ///< V: the packet lies past the row
@@ -44,24 +45,58 @@ struct columns {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int own = (l + k * G) * V;
-      const bool active = own < experts;
-      at[k] = own + V <= experts ? own : active ? experts - V : 0;
+      const bool active = FULL || own < experts;
+      at[k] = FULL || own + V <= experts ? own : active ? experts - V : 0;
       skip[k] = active ? own - at[k] : V;
     }
   }
+  __device__ __forceinline__ bool mine(int k, int e) const { return FULL || e >= skip[k]; }
 };
 
-template <int G>
-__device__ __forceinline__ float row_max(float v) {
-#pragma unroll
-  for (int d = G / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, wave::size));
+/// v of the lane that differs in bit log2(D) of its number where the lanes below D agree: a step of a reduction over 2 D lanes.  Within
+/// 16 lanes by DPP, beyond by gfx950's row swaps: no LDS traffic.
+template <int D>
+__device__ __forceinline__ void partner(float v, float& a, float& b) {
+  const int i = __builtin_bit_cast(int, v);
+  if constexpr (D < 16) {
+    constexpr int ctrl = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;  // quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror, row_mirror
+    a = v;
+    b = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, ctrl, 0xF, 0xF, true));
+  } else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+    a = __builtin_bit_cast(float, static_cast<int>(r[0]));
+    b = __builtin_bit_cast(float, static_cast<int>(r[1]));
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(i, i, false, false);
+    a = __builtin_bit_cast(float, static_cast<int>(r[0]));
+    b = __builtin_bit_cast(float, static_cast<int>(r[1]));
+  }
+}
+/// Over G adjacent lanes, the result in all of them.
+template <int G, typename F>
+__device__ __forceinline__ float row_reduce(float v, F&& f) {
+  float a, b;
+  const auto step = [&](auto d) {
+    if constexpr (decltype(d)::value < G) {
+      partner<decltype(d)::value>(v, a, b);
+      v = f(a, b);
+    }
+  };
+  step(std::integral_constant<int, 1>{});
+  step(std::integral_constant<int, 2>{});
+  step(std::integral_constant<int, 4>{});
+  step(std::integral_constant<int, 8>{});
+  step(std::integral_constant<int, 16>{});
+  step(std::integral_constant<int, 32>{});
   return v;
 }
 template <int G>
+__device__ __forceinline__ float row_max(float v) {
+  return row_reduce<G>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int G>
 __device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int d = G / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, wave::size);
-  return v;
+  return row_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 
 template <typename type_t, int V, int K>
@@ -69,42 +104,42 @@ struct row_packets {
   elements::packet_t<type_t, V> p[K];
 };
 
-template <int V, int G, int K, typename type_t>
-__device__ __forceinline__ row_packets<type_t, V, K> read_row(const type_t* __restrict__ row, const columns<V, G, K>& c) {
-  row_packets<type_t, V, K> r;
+template <typename type_t, typename cols_t, int V, int K>
+__device__ __forceinline__ void read_row(const type_t* __restrict__ row, const cols_t& c, row_packets<type_t, V, K>& r) {
 #pragma unroll
   for (int k = 0; k < K; ++k) r.p[k] = elements::load<V>(row + c.at[k]);
-  return r;
 }
 
-/// The lane's part of softmax(row); columns that are not the lane's get 0.
-template <int V, int G, int K, typename type_t>
-__device__ __forceinline__ void softmax(const row_packets<type_t, V, K>& r, const columns<V, G, K>& c, float (&p)[K][V]) {
+/// p = exp(row - its maximum) in the lane's columns (0 in columns that are not its own); returns the factor that makes it the softmax.  A row
+/// that takes no part is read as zeros and has the factor 0: what it holds (NaN) reaches nothing.
+/// (x - top, then times log2(e): one fma of x would save an instruction, but its rounding of top log2(e) is not small in a row at the type's
+/// lowest value.)
+template <int G, typename cols_t, typename type_t, int V, int K>
+__device__ __forceinline__ float exponentials(row_packets<type_t, V, K>& r, bool in, const cols_t& c, float (&p)[K][V]) {
   constexpr float lowest = -__builtin_inff();
   float top = lowest;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
+    if (!in) r.p[k] = elements::packet_t<type_t, V>{};
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      p[k][e] = e >= c.skip[k] ? static_cast<float>(r.p[k][e]) : lowest;
+      p[k][e] = c.mine(k, e) ? static_cast<float>(r.p[k][e]) : lowest;
       top = fmaxf(top, p[k][e]);
     }
+  }
   top = row_max<G>(top);
   if (top == lowest) top = 0.0f;  // nothing but -infinity (or NaN): exp gives 0 (NaN)
+  constexpr float log2e = 1.44269504088896340736f;
   float sum = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      p[k][e] = __expf(p[k][e] - top);
+      p[k][e] = __builtin_amdgcn_exp2f((p[k][e] - top) * log2e);
       sum += p[k][e];
     }
   sum = row_sum<G>(sum);
-  const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int e = 0; e < V; ++e) p[k][e] *= scale;
+  return !in || sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum);
 }
 
 /// Sum over the workgroup, in a fixed order, in every thread (`scratch`: one float per wavefront).
@@ -143,35 +178,29 @@ struct outputs {
 };
 
 namespace detail {
-/// Thread e < experts brings column e's sum of probabilities and its count.
-__device__ __forceinline__ void finish(float sum, int count, int tokens, int experts, int choices, float coefficient, const outputs& out,
-                                       float* __restrict__ scratch) {
-  const int e = threadIdx.x;
+/// Writes column e's outputs and returns its term of the loss.
+__device__ __forceinline__ float finish_column(int e, float sum, int count, int tokens, int experts, int choices, const outputs& out) {
+  if (e >= experts) return 0.0f;
   const float per_token = tokens > 0 ? 1.0f / static_cast<float>(tokens) : 0.0f;
-  float term = 0.0f;
-  if (e < experts) {
-    const float probability = sum * per_token;
-    out.counts[e] = count;
-    out.probability[e] = probability;
-    term = static_cast<float>(count) * per_token / static_cast<float>(choices) * probability;
-  }
-  const float all = block_sum(term, scratch);
-  if (threadIdx.x == 0) {
-    *out.loss = coefficient * static_cast<float>(experts) * all;
-    *out.tokens = tokens;
-  }
+  const float probability = sum * per_token;
+  out.counts[e] = count;
+  out.probability[e] = probability;
+  return static_cast<float>(count) * per_token / static_cast<float>(choices) * probability;
 }
 }  // namespace detail
 
+/// Floats (ints) between the partial sums (counts) of two workgroups: whole 64-column groups, 16-byte aligned.
+__host__ __device__ constexpr int partial_pitch(int experts) { return (experts + wave::size - 1) / wave::size * wave::size; }
+
 /**
  * Workgroup b reads tokens [b per, (b + 1) per): G lanes share a row, each keeps the sums of its own columns in registers over all of its
- * rows.  ONE: the only workgroup finishes as well; otherwise it leaves sums[b][experts], counts[b][experts], tokens[b].
+ * rows.  ONE: the only workgroup finishes as well; otherwise it leaves sums[b], counts[b] (rows of partial_pitch) and counted[b].
  */
-template <bool ONE, int V, int G, int K, int U, typename type_t, typename id_t>
+template <bool ONE, bool FULL, int V, int G, int K, int U, typename type_t, typename id_t>
 __global__ void __launch_bounds__(threads)
 forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* __restrict__ chosen, const unsigned char* __restrict__ mask,
         const int tokens, const int experts, const int choices, const int per, const float coefficient, const outputs out,
-        float* __restrict__ sums, int* __restrict__ counts, int* __restrict__ counted) {
+        float* __restrict__ sums, int* __restrict__ counts, int* __restrict__ counted, int* __restrict__ finished) {
   constexpr int rows_per_wave = wave::size / G;
   constexpr int rows_per_step = rows_per_wave * waves;
   __shared__ float s_sum[waves][K * G * V];
@@ -186,33 +215,40 @@ forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* 
   const long long begin = static_cast<long long>(blockIdx.x) * per;
   const long long end = begin + per < tokens ? begin + per : tokens;
 
-  const detail::columns<V, G, K> cols(experts);
+  const detail::columns<FULL, V, G, K> cols(experts);
   float sum[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[k][e] = 0.0f;
   int mine = 0;
-  for (long long t0 = begin + w * rows_per_wave + wave::lane() / G; t0 < end; t0 += U * rows_per_step) {
+  const int last = static_cast<int>(end);
+  int t0 = static_cast<int>(begin) + w * rows_per_wave + wave::lane() / G;
+  const type_t* __restrict__ row = logits + static_cast<std::size_t>(t0) * pitch;
+  const std::size_t step = static_cast<std::size_t>(rows_per_step) * pitch;
+  for (; t0 < last; t0 += U * rows_per_step, row += U * step) {
     detail::row_packets<type_t, V, K> r[U];
+    unsigned char counts_in[U];
     bool in[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long t = t0 + u * rows_per_step;
-      in[u] = t < end;
-      const long long from = in[u] ? t : t0;
-      r[u] = detail::read_row<V, G, K>(logits + from * pitch, cols);
-      if (mask) in[u] = in[u] && mask[from] != 0;
+    for (int u = 0; u < U; ++u) counts_in[u] = 1;
+    if (mask) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) counts_in[u] = mask[t0 + u * rows_per_step < last ? t0 + u * rows_per_step : t0];
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) detail::read_row(t0 + u * rows_per_step < last ? row + u * step : row, cols, r[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) in[u] = t0 + u * rows_per_step < last && counts_in[u] != 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float p[K][V];
-      detail::softmax<V, G, K>(r[u], cols, p);
+      const float scale = detail::exponentials<G>(r[u], in[u], cols, p);
       mine += in[u] ? 1 : 0;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum[k][e] += in[u] ? p[k][e] : 0.0f;
+        for (int e = 0; e < V; ++e) sum[k][e] = __builtin_fmaf(p[k][e], scale, sum[k][e]);
     }
   }
   detail::count_choices(chosen, mask, choices, begin, end, experts, s_count);
@@ -229,103 +265,113 @@ forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* 
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (e >= cols.skip[k]) s_sum[w][cols.at[k] + e] = sum[k][e];
+        if (cols.mine(k, e)) s_sum[w][cols.at[k] + e] = sum[k][e];
   }
   __syncthreads();
   float total = 0.0f;
   if (tid < experts)
     for (int i = 0; i < waves; ++i) total += s_sum[i][tid];
   if constexpr (ONE) {
-    detail::finish(total, tid < experts ? s_count[tid] : 0, s_tokens, experts, choices, coefficient, out, s_scratch);
+    const float term = detail::finish_column(tid, total, tid < experts ? s_count[tid] : 0, s_tokens, experts, choices, out);
+    const float loss = detail::block_sum(term, s_scratch);
+    if (tid == 0) {
+      *out.loss = coefficient * static_cast<float>(experts) * loss;
+      *out.tokens = s_tokens;
+    }
   } else {
     if (tid < experts) {
-      sums[static_cast<std::size_t>(blockIdx.x) * experts + tid] = total;
-      counts[static_cast<std::size_t>(blockIdx.x) * experts + tid] = s_count[tid];
+      sums[static_cast<std::size_t>(blockIdx.x) * partial_pitch(experts) + tid] = total;
+      counts[static_cast<std::size_t>(blockIdx.x) * partial_pitch(experts) + tid] = s_count[tid];
     }
-    if (tid == 0) counted[blockIdx.x] = s_tokens;
+    if (tid == 0) {
+      counted[blockIdx.x] = s_tokens;
+      if (blockIdx.x == 0) *finished = 0;
+    }
   }
 }
 
-/// Adds the workgroups' sums up: 4 columns per thread, the workgroups dealt out to slices of the threads and added in a fixed order.
+/**
+ * Adds the workgroups' sums up, in a fixed order: a workgroup takes 64 columns, 4 per thread, and deals the `groups` out to 64 slices of its
+ * threads.  Its part of the loss goes into parts[blockIdx.x]; the workgroup that counts itself last in *finished (0 at the start: the
+ * forward kernel cleared it) adds the parts up.  No workgroup waits for another.
+ */
 template <typename = void>
 __global__ void __launch_bounds__(threads)
 finish_forward(const float* __restrict__ sums, const int* __restrict__ counts, const int* __restrict__ counted, const int groups, const int experts,
-               const int choices, const float coefficient, const outputs out) {
-  constexpr int C = 4, U = 8;
-  __shared__ float s_sum[threads * C];
-  __shared__ int s_count[threads * C];
-  __shared__ float s_scratch[waves];
+               const int choices, const float coefficient, const outputs out, float* __restrict__ parts, int* __restrict__ finished) {
+  constexpr int C = 4;
+  constexpr int width = wave::size / C;  // threads across the columns
+  constexpr int slices = threads / width;
+  __shared__ float s_sum[slices][wave::size];
+  __shared__ int s_count[slices][wave::size];
   __shared__ int s_tokens;
   const int tid = threadIdx.x;
-  int width = 1;  // threads per slice
-  while (width * C < experts) width *= 2;
-  const int slices = threads / width;
-  const int column = tid % width * C;
-  const int mine = column < experts ? (experts - column < C ? experts - column : C) : 0;
+  const int slice = tid / width;
+  const int local = tid % width * C;
+  const int column = static_cast<int>(blockIdx.x) * wave::size + local;
   if (tid == 0) s_tokens = 0;
-  float sum[C] = {0.0f, 0.0f, 0.0f, 0.0f};
-  int count[C] = {0, 0, 0, 0};
-  if (mine > 0) {
-    for (int b0 = tid / width; b0 < groups; b0 += slices * U) {
-      float v[U][C];
-      int n[U][C];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int b = b0 + u * slices < groups ? b0 + u * slices : b0;
-        const std::size_t at = static_cast<std::size_t>(b) * experts + column;
-        if (mine == C) {
-          const auto x = elements::load<C>(sums + at);
-          const auto y = elements::load<C>(counts + at);
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            v[u][c] = x[c];
-            n[u][c] = y[c];
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            v[u][c] = c < mine ? sums[at + c] : 0.0f;
-            n[u][c] = c < mine ? counts[at + c] : 0;
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (b0 + u * slices < groups) {
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            sum[c] += v[u][c];
-            count[c] += n[u][c];
-          }
-        }
-    }
+  typedef float real_t __attribute__((ext_vector_type(C)));
+  typedef int whole_t __attribute__((ext_vector_type(C)));
+  real_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  whole_t count = {0, 0, 0, 0};
+  const int pitch = partial_pitch(experts);  // (columns past the last expert are read, and dropped)
+#pragma unroll 8
+  for (int b = slice; b < groups; b += slices) {
+    const std::size_t at = static_cast<std::size_t>(b) * pitch + column;
+    sum += *reinterpret_cast<const real_t*>(sums + at);
+    count += *reinterpret_cast<const whole_t*>(counts + at);
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    s_sum[tid * C + c] = sum[c];
-    s_count[tid * C + c] = count[c];
+    s_sum[slice][local + c] = sum[c];
+    s_count[slice][local + c] = count[c];
   }
   __syncthreads();
   if (tid < groups) atomicAdd(&s_tokens, counted[tid]);
+  // 64 slices to 16 to one
+  constexpr int fold = slices / waves;
+  const int w = tid / wave::size, lane = wave::lane();
   float total = 0.0f;
   int all = 0;
-  if (tid < experts)
-    for (int i = 0; i < slices; ++i) {
-      total += s_sum[i * width * C + tid];
-      all += s_count[i * width * C + tid];
-    }
+#pragma unroll
+  for (int i = 0; i < fold; ++i) {
+    total += s_sum[w * fold + i][lane];
+    all += s_count[w * fold + i][lane];
+  }
   __syncthreads();
-  detail::finish(total, all, s_tokens, experts, choices, coefficient, out, s_scratch);
+  s_sum[w][lane] = total;
+  s_count[w][lane] = all;
+  __syncthreads();
+  if (w == 0) {
+#pragma unroll
+    for (int i = 1; i < waves; ++i) {
+      total += s_sum[i][lane];
+      all += s_count[i][lane];
+    }
+    const int e = static_cast<int>(blockIdx.x) * wave::size + lane;
+    const float part = detail::finish_column(e, total, all, s_tokens, experts, choices, out);
+    const float loss = detail::row_sum<wave::size>(part);
+    if (lane == 0) {
+      __hip_atomic_store(parts + blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int before = __hip_atomic_fetch_add(finished, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+      if (before == static_cast<int>(gridDim.x) - 1) {
+        float sum_of_parts = 0.0f;
+        for (unsigned int i = 0; i < gridDim.x; ++i) sum_of_parts += __hip_atomic_load(parts + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *out.loss = coefficient * static_cast<float>(experts) * sum_of_parts;
+        *out.tokens = s_tokens;
+      }
+    }
+  }
 }
 
 /// Gradient of the logits: G lanes share a row, which is read, turned into probabilities and written within the registers.
-template <int V, int G, int K, int U, typename type_t>
+template <bool FULL, int V, int G, int K, int U, typename type_t>
 __global__ void __launch_bounds__(256)
 backward(const type_t* __restrict__ logits, const std::size_t pitch, const int* __restrict__ counts, const int* __restrict__ counted,
          const unsigned char* __restrict__ mask, const int tokens, const int experts, const int choices, const float coefficient,
          const float* __restrict__ grad_loss, type_t* __restrict__ grad, const std::size_t grad_pitch) {
   constexpr int rows_per_wave = wave::size / G;
-  const detail::columns<V, G, K> cols(experts);
+  const detail::columns<FULL, V, G, K> cols(experts);
   const int n = *counted;
   const float per_token = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
   const float scale = (grad_loss ? *grad_loss : 1.0f) * coefficient * static_cast<float>(experts) * per_token;
@@ -334,42 +380,51 @@ backward(const type_t* __restrict__ logits, const std::size_t pitch, const int* 
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int e = 0; e < V; ++e) weight[k][e] = e >= cols.skip[k] ? static_cast<float>(counts[cols.at[k] + e]) * share : 0.0f;
-  const long long stride = static_cast<long long>(gridDim.x) * (4 * rows_per_wave);
-  for (long long t0 = static_cast<long long>(blockIdx.x) * (4 * rows_per_wave) + threadIdx.x / G; t0 < tokens; t0 += stride * U) {
+    for (int e = 0; e < V; ++e) weight[k][e] = cols.mine(k, e) ? static_cast<float>(counts[cols.at[k] + e]) * share : 0.0f;
+  const unsigned int count = static_cast<unsigned int>(tokens);
+  const unsigned int stride = gridDim.x * (4 * rows_per_wave);
+  unsigned int t0 = blockIdx.x * (4 * rows_per_wave) + threadIdx.x / G;
+  const type_t* __restrict__ row = logits + static_cast<std::size_t>(t0) * pitch;
+  type_t* __restrict__ to_row = grad + static_cast<std::size_t>(t0) * grad_pitch;
+  const std::size_t step = static_cast<std::size_t>(stride) * pitch, to_step = static_cast<std::size_t>(stride) * grad_pitch;
+  for (; t0 < count; t0 += stride * U, row += U * step, to_row += U * to_step) {
     detail::row_packets<type_t, V, K> r[U];
+    unsigned char counts_in[U];
     bool in[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long t = t0 + u * stride;
-      const long long from = t < tokens ? t : t0;
-      in[u] = !mask || mask[from] != 0;
-      r[u] = detail::read_row<V, G, K>(logits + from * pitch, cols);
+    for (int u = 0; u < U; ++u) counts_in[u] = 1;
+    if (mask) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) counts_in[u] = mask[t0 + u * stride < count ? t0 + u * stride : t0];
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) detail::read_row(t0 + u * stride < count ? row + u * step : row, cols, r[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) in[u] = counts_in[u] != 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float p[K][V];
-      detail::softmax<V, G, K>(r[u], cols, p);
+      const float factor = detail::exponentials<G>(r[u], in[u], cols, p);
       float dot = 0.0f;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int e = 0; e < V; ++e) dot += p[k][e] * weight[k][e];
-      dot = detail::row_sum<G>(dot);
-      const long long t = t0 + u * stride;
-      if (t < tokens) {
-        type_t* const to = grad + t * grad_pitch;
+        for (int e = 0; e < V; ++e) dot = __builtin_fmaf(p[k][e], weight[k][e], dot);
+      dot = detail::row_sum<G>(dot) * factor;
+      const float by = factor == 0.0f ? 0.0f : factor * scale;  // (also for an upstream gradient that is not finite)
+      if (t0 + u * stride < count) {
+        type_t* const to = to_row + u * to_step;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           float g[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) g[e] = in[u] ? p[k][e] * (weight[k][e] - dot) * scale : 0.0f;
-          if (cols.skip[k] == 0) {
+          for (int e = 0; e < V; ++e) g[e] = p[k][e] * by * (weight[k][e] - dot);
+          if (FULL || cols.skip[k] == 0) {
             elements::store<V>(to + cols.at[k], g);
           } else {
 #pragma unroll
             for (int e = 0; e < V; ++e)
-              if (e >= cols.skip[k]) to[cols.at[k] + e] = static_cast<type_t>(g[e]);
+              if (cols.mine(k, e)) to[cols.at[k] + e] = static_cast<type_t>(g[e]);
           }
         }
       }
@@ -431,29 +486,35 @@ inline groups_t share_out(int tokens, long long work_per_token, long long least,
 inline groups_t forward_groups(int tokens, int experts) { return share_out(tokens, experts, static_cast<long long>(tokens) * experts <= 32768 ? 32768 : 16384, max_groups); }
 inline groups_t count_groups(int tokens, int choices) { return share_out(tokens, choices, 16384, max_groups); }
 
+inline int finish_groups(int experts) { return (experts + wave::size - 1) / wave::size; }
+/// sums[groups][pitch], counts[groups][pitch], counted[groups], parts[finish_groups], finished[1].
 inline std::size_t forward_workspace_bytes(int tokens, int experts) {
   const groups_t g = forward_groups(tokens, experts);
-  return g.groups == 1 ? 0 : static_cast<std::size_t>(g.groups) * (2 * static_cast<std::size_t>(experts) + 1) * 4;
+  return g.groups == 1 ? 0 : (static_cast<std::size_t>(g.groups) * (2 * static_cast<std::size_t>(partial_pitch(experts)) + 1) + finish_groups(experts) + 1) * 4;
 }
 inline std::size_t count_workspace_bytes(int tokens, int choices, int experts) {
   const groups_t g = count_groups(tokens, choices);
   return g.groups == 1 ? 0 : static_cast<std::size_t>(g.groups) * experts * sizeof(int);
 }
 
-/// Calls f(V, G, K) as integral constants: lanes per row and packets per lane for rows of `experts` values.
+/// Calls f(FULL, V, G, K) as integral constants: lanes per row and packets per lane for rows of `experts` values.
 template <typename type_t, typename F>
 void with_shape(int experts, F&& f) {
   constexpr int V = elements::per_access<type_t>;
   using one = std::integral_constant<int, 1>;
-  using v = std::integral_constant<int, V>;
+  const auto with = [&](auto v, auto lanes, auto k) {
+    if (experts == decltype(v)::value * decltype(lanes)::value * decltype(k)::value) f(std::true_type{}, v, lanes, k);
+    else f(std::false_type{}, v, lanes, k);
+  };
+  const std::integral_constant<int, V> v{};
   const int packets = (experts + V - 1) / V;
-  if (experts < V) f(one{}, std::integral_constant<int, 8>{}, one{});
-  else if (packets <= 8) f(v{}, std::integral_constant<int, 8>{}, one{});
-  else if (packets <= 16) f(v{}, std::integral_constant<int, 16>{}, one{});
-  else if (packets <= 32) f(v{}, std::integral_constant<int, 32>{}, one{});
-  else if (packets <= 64) f(v{}, std::integral_constant<int, 64>{}, one{});
-  else if (packets <= 128) f(v{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-  else if constexpr (sizeof(type_t) == 4) f(v{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  if (experts < V) f(std::false_type{}, one{}, std::integral_constant<int, 8>{}, one{});
+  else if (packets <= 8) with(v, std::integral_constant<int, 8>{}, one{});
+  else if (packets <= 16) with(v, std::integral_constant<int, 16>{}, one{});
+  else if (packets <= 32) with(v, std::integral_constant<int, 32>{}, one{});
+  else if (packets <= 64) with(v, std::integral_constant<int, 64>{}, one{});
+  else if (packets <= 128) with(v, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  else if constexpr (sizeof(type_t) == 4) with(v, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
 }
 
 template <typename type_t, typename id_t>
@@ -461,18 +522,22 @@ int launch_forward(hipStream_t stream, const type_t* logits, std::size_t pitch, 
                    int choices, float coefficient, const outputs& out, void* workspace) {
   const groups_t g = forward_groups(tokens, experts);
   float* const sums = static_cast<float*>(workspace);
-  int* const counts = reinterpret_cast<int*>(sums + static_cast<std::size_t>(g.groups) * experts);
-  int* const counted = counts + static_cast<std::size_t>(g.groups) * experts;
-  with_shape<type_t>(experts, [&](auto v, auto lanes, auto k) {
+  int* const counts = reinterpret_cast<int*>(sums + static_cast<std::size_t>(g.groups) * partial_pitch(experts));
+  int* const counted = counts + static_cast<std::size_t>(g.groups) * partial_pitch(experts);
+  float* const parts = reinterpret_cast<float*>(counted + g.groups);
+  int* const finished = reinterpret_cast<int*>(parts + finish_groups(experts));
+  with_shape<type_t>(experts, [&](auto full, auto v, auto lanes, auto k) {
+    constexpr bool FULL = decltype(full)::value;
     constexpr int V = decltype(v)::value, G = decltype(lanes)::value, K = decltype(k)::value, U = K == 1 ? 2 : 1;
     if (g.groups == 1)
-      forward<true, V, G, K, U, type_t, id_t><<<1, threads, 0, stream>>>(logits, pitch, chosen, mask, tokens, experts, choices, g.per, coefficient, out,
-                                                                       nullptr, nullptr, nullptr);
+      forward<true, FULL, V, G, K, U, type_t, id_t><<<1, threads, 0, stream>>>(logits, pitch, chosen, mask, tokens, experts, choices, g.per, coefficient, out,
+                                                                       nullptr, nullptr, nullptr, nullptr);
     else
-      forward<false, V, G, K, U, type_t, id_t><<<g.groups, threads, 0, stream>>>(logits, pitch, chosen, mask, tokens, experts, choices, g.per,
-                                                                               coefficient, out, sums, counts, counted);
+      forward<false, FULL, V, G, K, U, type_t, id_t><<<g.groups, threads, 0, stream>>>(logits, pitch, chosen, mask, tokens, experts, choices, g.per,
+                                                                               coefficient, out, sums, counts, counted, finished);
   });
-  if (g.groups > 1) finish_forward<><<<1, threads, 0, stream>>>(sums, counts, counted, g.groups, experts, choices, coefficient, out);
+  if (g.groups > 1)
+    finish_forward<><<<finish_groups(experts), threads, 0, stream>>>(sums, counts, counted, g.groups, experts, choices, coefficient, out, parts, finished);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -480,12 +545,13 @@ template <typename type_t>
 int launch_backward(hipStream_t stream, const type_t* logits, std::size_t pitch, const int* counts, const int* counted, const unsigned char* mask,
                     int tokens, int experts, int choices, float coefficient, const float* grad_loss, type_t* grad, std::size_t grad_pitch) {
   if (tokens == 0) return 0;
-  with_shape<type_t>(experts, [&](auto v, auto lanes, auto k) {
+  with_shape<type_t>(experts, [&](auto full, auto v, auto lanes, auto k) {
+    constexpr bool FULL = decltype(full)::value;
     constexpr int V = decltype(v)::value, G = decltype(lanes)::value, K = decltype(k)::value, U = K == 1 ? 2 : 1;
     constexpr int rows = 4 * (wave::size / G);
     const long long groups = (static_cast<long long>(tokens) + rows - 1) / rows;
-    const unsigned int grid = static_cast<unsigned int>(groups < 2048 ? groups : 2048);
-    backward<V, G, K, U, type_t><<<grid, 256, 0, stream>>>(logits, pitch, counts, counted, mask, tokens, experts, choices, coefficient, grad_loss, grad,
+    const unsigned int grid = static_cast<unsigned int>(groups < 8192 ? groups : 8192);
+    backward<FULL, V, G, K, U, type_t><<<grid, 256, 0, stream>>>(logits, pitch, counts, counted, mask, tokens, experts, choices, coefficient, grad_loss, grad,
                                                           grad_pitch);
   });
   return static_cast<int>(hipGetLastError());
