@@ -201,7 +201,10 @@ __device__ __forceinline__ int same_key(const int* __restrict__ keys, int tokens
   return __popcll(__ballot(j >= 0 && j < tokens && keys[j < 0 ? 0 : j < tokens ? j : tokens - 1] == key));
 }
 
-/// A position that group_ids did not write stays inside the array.
+/// Ids and positions that group_ids did not write are not followed out of the arrays, whatever they are: positions are bounded, ids count
+/// up to the first that is no row (`leading` of the lanes that hold one).
+__device__ __forceinline__ bool is_row(int key, int rows) { return static_cast<unsigned int>(key) < static_cast<unsigned int>(rows); }
+__device__ __forceinline__ int leading(unsigned long long lanes) { return lanes == ~0ull ? wave::size : __builtin_ctzll(~lanes); }
 __device__ __forceinline__ int bounded(int position, int tokens) {
   return static_cast<unsigned int>(position) < static_cast<unsigned int>(tokens) ? position : 0;
 }
@@ -225,7 +228,7 @@ gradient_overwrite(const int* __restrict__ keys, const int* __restrict__ positio
   const long long d0 = static_cast<long long>(tile) * items;
   const long long d1 = d0 + items < total ? d0 + items : total;
   int y = __builtin_amdgcn_readfirstlane(tokens_before(keys, tokens, d0));
-  int row = static_cast<int>(d0 - y);
+  int row = d0 > y ? static_cast<int>(d0 - y) : 0;
   bool open = false;  // the row was begun by an earlier tile, and is cut here
   if (y > 0 && row < rows && keys[y - 1] == row) {
     const int behind = same_key<false>(keys, tokens, y, row);
@@ -293,8 +296,7 @@ gradient_overwrite(const int* __restrict__ keys, const int* __restrict__ positio
       key = keys[j];
       position = bounded(positions[j], tokens);
     }
-    const bool mine = key < rows && static_cast<long long>(j) + key < d1;  // (a prefix of the lanes)
-    const int count = __popcll(__ballot(mine));
+    const int count = leading(__ballot(is_row(key, rows) && static_cast<long long>(j) + key < d1));
     consume(key, position, count);
     if (count < wave::size) {
       next_key = __builtin_amdgcn_readlane(key, count);
@@ -311,7 +313,7 @@ gradient_overwrite(const int* __restrict__ keys, const int* __restrict__ positio
   bool unfinished = open || y > begun;
   if (unfinished && !open) {
     const int behind = next_key == row ? same_key<false>(keys, tokens, y, row) : 0;
-    if (y - begun + behind < whole_row) {  // a short row is finished here
+    if (y - begun + behind < whole_row && row < rows) {  // a short row is finished here
       const int j = y + wave::lane();
       consume(row, j < tokens ? bounded(positions[j], tokens) : 0, behind);
       finish();
@@ -342,7 +344,7 @@ gradient_add(const int* __restrict__ keys, const int* __restrict__ positions, co
   const int end = d0 + items < tokens ? static_cast<int>(d0 + items) : tokens;
   int row = keys[y];
   bool open = false;  // the row was begun by an earlier tile, and is cut here
-  if (y > 0 && row < rows && keys[y - 1] == row) {
+  if (y > 0 && is_row(row, rows) && keys[y - 1] == row) {
     const int behind = same_key<false>(keys, tokens, y, row);
     open = same_key<true>(keys, tokens, y, row) + behind >= whole_row;
     if (!open) y += behind;
@@ -398,7 +400,7 @@ gradient_add(const int* __restrict__ keys, const int* __restrict__ positions, co
       position = bounded(positions[j], tokens);
       if (j + 1 < tokens) next = keys[j + 1];
     }
-    const int count = __popcll(__ballot(key < rows && j < end));
+    const int count = leading(__ballot(is_row(key, rows) && j < end));
     if (count == 0) break;
     const unsigned long long last = __ballot(key != next);
     row = __builtin_amdgcn_readlane(key, count - 1);
@@ -449,7 +451,7 @@ gradient_add_small(const int* __restrict__ keys, const int* __restrict__ positio
     position = bounded(positions[j], tokens);
     if (j + 1 < tokens) next = keys[j + 1];
   }
-  const int count = __popcll(__ballot(key < rows));
+  const int count = leading(__ballot(is_row(key, rows)));
   const unsigned long long last = __ballot(key != next);
   bool open = count > 0 && begin > 0 && keys[begin - 1] == __builtin_amdgcn_readfirstlane(key);
   int head_row = -1;

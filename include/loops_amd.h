@@ -580,7 +580,7 @@ int loops_allgatherv_f64(void* comm, int rank, int world, double* y_full, const 
  * returns LOOPS_E_CONFIG.  Matrices are row-major with unit column stride; a pitch is the distance of two rows in elements (>= the
  * row's width, LOOPS_E_BADARG otherwise), at any alignment of the element.  An output that overlaps an input (by the
  * addresses between their first and last elements) is LOOPS_E_BADARG.
- * `first_id` (>= 0): the id of the table's row 0.  A token whose id is outside [first_id, first_id + rows) -- padding, or a row that
+ * `first_id` (>= 0, first_id + rows within long long): the id of the table's row 0.  A token whose id is outside [first_id, first_id + rows) -- padding, or a row that
  * another rank's shard of the table holds -- has a zero row in the lookup and no part in the gradient; no id is an error.
  * Calls are asynchronous and may be captured; they keep nothing between calls: scratch memory is the caller's `workspace`
  * (hipMalloc'd, 16-byte aligned, at least what the *_workspace function says for the same sizes, LOOPS_E_BADARG otherwise; it may be

@@ -8,6 +8,7 @@
 #include <loops_amd.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdint>
 #include <cstdlib>
 #include <limits>

@@ -63,6 +63,16 @@ def pitch_of(t: torch.Tensor, what: str) -> int:
     return pitch
 
 
+INT_MAX = 2 ** 31 - 1
+LONG_MAX = 2 ** 63 - 1
+
+
+def c_int(name: str, *sizes: int) -> None:
+    """Refuses sizes that the C entry point's int arguments do not hold."""
+    if max(sizes) > INT_MAX or min(sizes) < -INT_MAX:
+        L.check(-2, name)
+
+
 _entries = {}
 
 
@@ -71,11 +81,14 @@ def launch(device: int, name: str, *args) -> None:
     fn = _entries.get(name)
     if fn is None:
         fn = _entries[name] = getattr(L.lib(), name)
-    if device == torch._C._cuda_getDevice():
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
+    try:
+        if device == torch._C._cuda_getDevice():
             code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        else:
+            with torch.cuda.device(device):
+                code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    except C.ArgumentError as e:
+        raise TypeError(f"{name}: {e}") from None
     if code:
         L.check(code, name)
 
@@ -105,11 +118,12 @@ def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, first_
     pitch = pitch_of(table, "table")
     if not tokens.is_contiguous():
         raise ValueError("tokens must be contiguous")
-    if first_id < 0:
-        raise ValueError("first_id must not be negative")
+    if not 0 <= first_id <= LONG_MAX:
+        raise ValueError("first_id must not be negative or beyond 64 bits")
     device = same_device(table, tokens, out)
     rows, dim = table.shape
     n = tokens.numel()
+    c_int("loops_embedding_lookup", n, rows, dim)
     if out is None:
         out = torch.empty(*tokens.shape, dim, dtype=table.dtype, device=device)
         out_pitch = dim
@@ -137,10 +151,11 @@ def group_tokens(tokens: torch.Tensor, rows: int, first_id: int = 0, drop_id: in
     index = index_type(tokens, "tokens")
     if not tokens.is_contiguous():
         raise ValueError("tokens must be contiguous")
-    if first_id < 0 or rows < 0:
-        raise ValueError("first_id and rows must not be negative")
+    if rows < 0 or not 0 <= first_id <= LONG_MAX or not -LONG_MAX <= drop_id <= LONG_MAX:
+        raise ValueError("first_id and rows must not be negative, ids not beyond 64 bits")
     device = same_device(tokens)
     n = tokens.numel()
+    c_int("loops_group_tokens", n, rows)
     _keep, ws, size = workspace(device, "loops_group_tokens_workspace", n, rows)
     ids = torch.empty(n, dtype=torch.int32, device=device)
     positions = torch.empty(n, dtype=torch.int32, device=device)
@@ -159,6 +174,10 @@ def gradient(groups: TokenGroups, grad: torch.Tensor, scale: float = 1.0, dtype:
     value = value_type(grad, "grad")
     ids, positions, rows = groups
     n = ids.numel()
+    if ids.dtype is not torch.int32 or positions.dtype is not torch.int32:
+        raise TypeError("groups must hold int32")
+    if positions.numel() != n or not ids.is_contiguous() or not positions.is_contiguous():
+        raise ValueError("groups must hold as many ids as positions, contiguous")
     if grad.dim() == 0:
         raise ValueError("grad must have the tokens' shape and a last dimension")
     dim = grad.shape[-1]
@@ -170,6 +189,7 @@ def gradient(groups: TokenGroups, grad: torch.Tensor, scale: float = 1.0, dtype:
         raise ValueError("grad must have a row for each token")
     pitch = pitch_of(grad, "grad")
     device = same_device(grad, ids, positions, out)
+    c_int("loops_embedding_gradient", n, rows, dim)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")

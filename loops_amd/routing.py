@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .embedding import index_type, launch, pitch_of, same_device, value_type, workspace
+from .embedding import c_int, index_type, launch, pitch_of, same_device, value_type, workspace
 
 
 def _mask(mask: Optional[torch.Tensor], tokens: int):
@@ -39,6 +39,7 @@ def expert_counts(chosen: torch.Tensor, experts: int, mask: Optional[torch.Tenso
     choices = chosen.shape[1] if chosen.dim() == 2 else 1
     device = same_device(chosen, mask)
     masked = _mask(mask, tokens)
+    c_int("loops_expert_counts", tokens, choices, experts)
     _keep, ws, size = workspace(device, "loops_expert_counts_workspace", tokens, choices, experts)
     counts = torch.empty(experts, dtype=torch.int32, device=device)
     launch(device, "loops_expert_counts", index, tokens, choices, chosen.data_ptr(), masked, experts, counts.data_ptr(), ws, size)
@@ -66,6 +67,7 @@ def balance_loss(logits: torch.Tensor, chosen: torch.Tensor, coefficient: float 
     choices = chosen.shape[1]
     device = same_device(logits, chosen, mask)
     masked = _mask(mask, tokens)
+    c_int("loops_balance_loss", tokens, experts, choices)
     _keep, ws, size = workspace(device, "loops_balance_loss_workspace", tokens, experts)
     loss = torch.empty((), dtype=torch.float32, device=device)
     counts = torch.empty(experts, dtype=torch.int32, device=device)
@@ -85,8 +87,13 @@ def balance_loss_backward(logits: torch.Tensor, forward: BalanceLoss, mask: Opti
     tokens, experts = logits.shape
     if forward.counts.shape != (experts,):
         raise ValueError("forward was made of another number of experts")
+    if forward.counts.dtype is not torch.int32 or forward.tokens.dtype is not torch.int32:
+        raise TypeError("forward must hold int32 counts")
+    if not forward.counts.is_contiguous() or forward.tokens.numel() != 1:
+        raise ValueError("forward must hold contiguous counts and one number of tokens")
     device = same_device(logits, forward.counts, forward.tokens, mask, grad_loss, out)
     masked = _mask(mask, tokens)
+    c_int("loops_balance_loss_backward", tokens, experts, forward.choices)
     upstream = None
     if grad_loss is not None:
         if grad_loss.dtype is not torch.float32:
