@@ -160,10 +160,19 @@ __device__ __forceinline__ void count_choices(const id_t* __restrict__ chosen, c
                                               long long end, int experts, int* __restrict__ counts) {
   const id_t* const from = chosen + begin * choices;
   const unsigned int n = static_cast<unsigned int>((end - begin) * choices);
-  for (unsigned int i = threadIdx.x; i < n; i += blockDim.x) {
-    const long long e = static_cast<long long>(from[i]);
-    const bool counts_in = !mask || mask[begin + i / static_cast<unsigned int>(choices)] != 0;
-    if (counts_in && e >= 0 && e < experts) atomicAdd(&counts[e], 1);
+  constexpr unsigned int U = 4;  // reads in flight
+  for (unsigned int i = threadIdx.x; i < n; i += U * blockDim.x) {
+    long long e[U];
+    unsigned char counts_in[U];
+#pragma unroll
+    for (unsigned int u = 0; u < U; ++u) {
+      const unsigned int at = i + u * blockDim.x < n ? i + u * blockDim.x : i;
+      e[u] = static_cast<long long>(from[at]);
+      counts_in[u] = mask ? mask[begin + at / static_cast<unsigned int>(choices)] : 1;
+    }
+#pragma unroll
+    for (unsigned int u = 0; u < U; ++u)
+      if (i + u * blockDim.x < n && counts_in[u] != 0 && e[u] >= 0 && e[u] < experts) atomicAdd(&counts[e[u]], 1);
   }
 }
 
@@ -189,7 +198,7 @@ __device__ __forceinline__ float finish_column(int e, float sum, int count, int 
 }
 }  // namespace detail
 
-/// Floats (ints) between the partial sums (counts) of two workgroups: whole 64-column groups, 16-byte aligned.
+/// Floats (ints) between the partial sums (counts) of two workgroups: whole groups of columns of the finish kernel.
 __host__ __device__ constexpr int partial_pitch(int experts) { return (experts + wave::size - 1) / wave::size * wave::size; }
 
 /**
@@ -215,6 +224,7 @@ forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* 
   const long long begin = static_cast<long long>(blockIdx.x) * per;
   const long long end = begin + per < tokens ? begin + per : tokens;
 
+  detail::count_choices(chosen, mask, choices, begin, end, experts, s_count);
   const detail::columns<FULL, V, G, K> cols(experts);
   float sum[K][V];
 #pragma unroll
@@ -251,7 +261,6 @@ forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* 
         for (int e = 0; e < V; ++e) sum[k][e] = __builtin_fmaf(p[k][e], scale, sum[k][e]);
     }
   }
-  detail::count_choices(chosen, mask, choices, begin, end, experts, s_count);
   // rows of a wavefront, then wavefronts, always in the same order
 #pragma unroll
   for (int d = G; d < wave::size; d <<= 1)
@@ -291,73 +300,94 @@ forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* 
 }
 
 /**
- * Adds the workgroups' sums up, in a fixed order: a workgroup takes 64 columns, 4 per thread, and deals the `groups` out to 64 slices of its
- * threads.  Its part of the loss goes into parts[blockIdx.x]; the workgroup that counts itself last in *finished (0 at the start: the
- * forward kernel cleared it) adds the parts up.  No workgroup waits for another.
+ * Adds the workgroups' sums up, in a fixed order: a workgroup takes 16 columns, 4 per thread, and deals the `groups` out to 256 slices of
+ * its threads (512 x 256: 8.0 us at 64 columns per workgroup, 7.6 at 16; launch, one round of reads and the two trips of the count).  Its part of the loss
+ * goes into parts[blockIdx.x]; the workgroup that counts itself last in *finished (0 at the start: the forward kernel cleared it) adds the
+ * parts up.  No workgroup waits for another.
  */
+constexpr int finish_columns = 16;
+static_assert(max_experts / finish_columns <= wave::size, "a lane per part of the loss");
+
 template <typename = void>
 __global__ void __launch_bounds__(threads)
 finish_forward(const float* __restrict__ sums, const int* __restrict__ counts, const int* __restrict__ counted, const int groups, const int experts,
                const int choices, const float coefficient, const outputs out, float* __restrict__ parts, int* __restrict__ finished) {
   constexpr int C = 4;
-  constexpr int width = wave::size / C;  // threads across the columns
+  constexpr int width = finish_columns / C;  // threads across the columns
   constexpr int slices = threads / width;
-  __shared__ float s_sum[slices][wave::size];
-  __shared__ int s_count[slices][wave::size];
+  constexpr int apart = finish_columns + C;  // (rows of LDS, a few banks apart)
+  __shared__ float s_sum[slices * apart];
+  __shared__ int s_count[slices * apart];
   __shared__ int s_tokens;
   const int tid = threadIdx.x;
   const int slice = tid / width;
   const int local = tid % width * C;
-  const int column = static_cast<int>(blockIdx.x) * wave::size + local;
   if (tid == 0) s_tokens = 0;
   typedef float real_t __attribute__((ext_vector_type(C)));
   typedef int whole_t __attribute__((ext_vector_type(C)));
   real_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
   whole_t count = {0, 0, 0, 0};
   const int pitch = partial_pitch(experts);  // (columns past the last expert are read, and dropped)
-#pragma unroll 8
+  const int from = static_cast<int>(blockIdx.x) * finish_columns + local;
   for (int b = slice; b < groups; b += slices) {
-    const std::size_t at = static_cast<std::size_t>(b) * pitch + column;
+    const std::size_t at = static_cast<std::size_t>(b) * pitch + from;
     sum += *reinterpret_cast<const real_t*>(sums + at);
     count += *reinterpret_cast<const whole_t*>(counts + at);
   }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    s_sum[slice][local + c] = sum[c];
-    s_count[slice][local + c] = count[c];
+    s_sum[slice * apart + local + c] = sum[c];
+    s_count[slice * apart + local + c] = count[c];
   }
   __syncthreads();
   if (tid < groups) atomicAdd(&s_tokens, counted[tid]);
-  // 64 slices to 16 to one
-  constexpr int fold = slices / waves;
-  const int w = tid / wave::size, lane = wave::lane();
+  // 256 slices to 64 (one column per thread), to 16 (4 of a wavefront's), to one
+  constexpr int per_wave = slices / waves;
+  constexpr int rows = wave::size / finish_columns;
+  const int w = tid / wave::size, column = tid % finish_columns, row = wave::lane() / finish_columns;
   float total = 0.0f;
   int all = 0;
 #pragma unroll
-  for (int i = 0; i < fold; ++i) {
-    total += s_sum[w * fold + i][lane];
-    all += s_count[w * fold + i][lane];
+  for (int i = row; i < per_wave; i += rows) {
+    total += s_sum[(w * per_wave + i) * apart + column];
+    all += s_count[(w * per_wave + i) * apart + column];
+  }
+  const auto fold = [&]() {
+#pragma unroll
+    for (int d = finish_columns; d < wave::size; d <<= 1) {
+      total += __shfl_xor(total, d, wave::size);
+      all += __shfl_xor(all, d, wave::size);
+    }
+  };
+  fold();
+  __syncthreads();
+  if (row == 0) {
+    s_sum[w * apart + column] = total;
+    s_count[w * apart + column] = all;
   }
   __syncthreads();
-  s_sum[w][lane] = total;
-  s_count[w][lane] = all;
-  __syncthreads();
   if (w == 0) {
+    total = 0.0f;
+    all = 0;
 #pragma unroll
-    for (int i = 1; i < waves; ++i) {
-      total += s_sum[i][lane];
-      all += s_count[i][lane];
+    for (int i = row; i < waves; i += rows) {
+      total += s_sum[i * apart + column];
+      all += s_count[i * apart + column];
     }
-    const int e = static_cast<int>(blockIdx.x) * wave::size + lane;
-    const float part = detail::finish_column(e, total, all, s_tokens, experts, choices, out);
-    const float loss = detail::row_sum<wave::size>(part);
-    if (lane == 0) {
-      __hip_atomic_store(parts + blockIdx.x, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int before = __hip_atomic_fetch_add(finished, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-      if (before == static_cast<int>(gridDim.x) - 1) {
-        float sum_of_parts = 0.0f;
-        for (unsigned int i = 0; i < gridDim.x; ++i) sum_of_parts += __hip_atomic_load(parts + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *out.loss = coefficient * static_cast<float>(experts) * sum_of_parts;
+    fold();
+    const int e = row == 0 ? static_cast<int>(blockIdx.x) * finish_columns + column : experts;
+    const float part = detail::row_sum<wave::size>(detail::finish_column(e, total, all, s_tokens, experts, choices, out));
+    int before = 0;
+    if (wave::lane() == 0) {
+      __hip_atomic_store(parts + blockIdx.x, part, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      before = __hip_atomic_fetch_add(finished, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (__builtin_amdgcn_readfirstlane(before) == static_cast<int>(gridDim.x) - 1) {
+      const int lane = wave::lane();
+      const float loss = detail::row_sum<wave::size>(
+          lane < static_cast<int>(gridDim.x) ? __hip_atomic_load(parts + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f);
+      if (lane == 0) {
+        *out.loss = coefficient * static_cast<float>(experts) * loss;
         *out.tokens = s_tokens;
       }
     }
@@ -484,9 +514,9 @@ inline groups_t share_out(int tokens, long long work_per_token, long long least,
 }
 /// One workgroup up to 32 768 logits.
 inline groups_t forward_groups(int tokens, int experts) { return share_out(tokens, experts, static_cast<long long>(tokens) * experts <= 32768 ? 32768 : 16384, max_groups); }
-inline groups_t count_groups(int tokens, int choices) { return share_out(tokens, choices, 16384, max_groups); }
+inline groups_t count_groups(int tokens, int choices) { return share_out(tokens, choices, 4096, max_groups); }
 
-inline int finish_groups(int experts) { return (experts + wave::size - 1) / wave::size; }
+inline int finish_groups(int experts) { return (experts + finish_columns - 1) / finish_columns; }
 /// sums[groups][pitch], counts[groups][pitch], counted[groups], parts[finish_groups], finished[1].
 inline std::size_t forward_workspace_bytes(int tokens, int experts) {
   const groups_t g = forward_groups(tokens, experts);

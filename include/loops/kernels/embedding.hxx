@@ -109,23 +109,19 @@ constexpr int lane_width = elements::per_access<type_t> < elements::per_access<o
 
 struct gradient_plan {
   int slabs;  ///< column slabs
-  int items;  ///< merge items per tile
+  int items;  ///< tokens per tile
   int tiles;
 };
 
-/**
- * The tokens, sorted by row, and the rows' ends form one merge list (overwriting: an empty row costs a store, as a token costs a
- * load), or the tokens alone do (adding: rows without a token are not touched).  Equal tiles of that list, one wavefront per (tile,
- * slab of columns); a row of a hundred thousand tokens and a hundred thousand empty rows are the same work per wavefront.
- */
-inline gradient_plan gradient_plan_for(int width, int tokens, int rows, int dim, bool add) {
+/// Equal tiles of the tokens sorted by row, one wavefront per (tile, slab of columns): a row of a hundred thousand tokens and a hundred
+/// thousand rows of one are the same work per wavefront.  16 384 wavefronts are two for every place on the chip.
+inline gradient_plan gradient_plan_for(int width, int tokens, int dim) {
   gradient_plan p;
   p.slabs = (dim + wave::size * width - 1) / (wave::size * width);
-  const long long total = static_cast<long long>(tokens) + (add ? 0 : rows);
-  long long items = (total * p.slabs + 16383) / 16384;
-  items = items < 8 ? 8 : items;
+  long long items = (static_cast<long long>(tokens) * p.slabs + 16383) / 16384;
+  items = items < 16 ? 16 : items;
   p.items = static_cast<int>(items);
-  p.tiles = static_cast<int>((total + items - 1) / items);
+  p.tiles = static_cast<int>((tokens + items - 1) / items);
   return p;
 }
 
@@ -136,28 +132,32 @@ struct tile_record {
   int tail_row;
 };
 
-constexpr int small_tokens = 1024;  ///< most tokens of gradient_add_small
+constexpr int small_tokens = 1024;  ///< most tokens of add_small
 
 /// Workspace: records[tiles], heads[tiles][dim], tails[tiles][dim] (float).
 inline std::size_t gradient_records_bytes(int tiles) { return (static_cast<std::size_t>(tiles) * sizeof(tile_record) + 255) & ~static_cast<std::size_t>(255); }
 template <typename type_t, typename out_t>
 std::size_t gradient_workspace_bytes(int tokens, int rows, int dim, bool add) {
   if (dim == 0 || rows == 0 || (add && tokens <= small_tokens)) return 0;
-  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, rows, dim, add);
+  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, dim);
   return gradient_records_bytes(p.tiles) + 2 * static_cast<std::size_t>(p.tiles) * dim * sizeof(float);
 }
 
-/// The number of tokens before merge position `at`: token j lies at j + key_j (the ends of the rows below key_j come first).  All
-/// lanes search together, 64 probes a step.
-__device__ __forceinline__ int tokens_before(const int* __restrict__ keys, int tokens, long long at) {
-  int lo = 0, hi = tokens;  // answer in [lo, hi]: first j with j + key_j >= at
+/// Ids and positions that group_ids did not write are not followed out of the arrays, whatever they are: positions are bounded, ids count
+/// up to the first that is no row (`leading` of the lanes that hold one).
+__device__ __forceinline__ bool is_row(int key, int rows) { return static_cast<unsigned int>(key) < static_cast<unsigned int>(rows); }
+__device__ __forceinline__ int leading(unsigned long long lanes) { return lanes == ~0ull ? wave::size : __builtin_ctzll(~lanes); }
+__device__ __forceinline__ int bounded(int position, int tokens) {
+  return static_cast<unsigned int>(position) < static_cast<unsigned int>(tokens) ? position : 0;
+}
+
+/// The number of keys below `row`.  All lanes search together, 64 probes a step.
+__device__ __forceinline__ int keys_below(const int* __restrict__ keys, int tokens, int row) {
+  int lo = 0, hi = tokens;  // answer in [lo, hi]
   while (hi > lo) {
-    const int size = hi - lo;
-    const int step = (size + wave::size - 1) / wave::size;
+    const int step = (hi - lo + wave::size - 1) / wave::size;
     const long long probe = static_cast<long long>(lo) + static_cast<long long>(wave::lane()) * step;
-    bool below = false;
-    if (probe < hi) below = probe + keys[probe] < at;
-    const int n = __popcll(__ballot(below));  // probes below are a prefix of the lanes
+    const int n = leading(__ballot(probe < hi && keys[probe < hi ? probe : lo] < row));
     if (n == 0) return lo;
     const long long next_hi = static_cast<long long>(lo) + static_cast<long long>(n) * step;
     lo = lo + (n - 1) * step + 1;
@@ -201,139 +201,101 @@ __device__ __forceinline__ int same_key(const int* __restrict__ keys, int tokens
   return __popcll(__ballot(j >= 0 && j < tokens && keys[j < 0 ? 0 : j < tokens ? j : tokens - 1] == key));
 }
 
-/// Ids and positions that group_ids did not write are not followed out of the arrays, whatever they are: positions are bounded, ids count
-/// up to the first that is no row (`leading` of the lanes that hold one).
-__device__ __forceinline__ bool is_row(int key, int rows) { return static_cast<unsigned int>(key) < static_cast<unsigned int>(rows); }
-__device__ __forceinline__ int leading(unsigned long long lanes) { return lanes == ~0ull ? wave::size : __builtin_ctzll(~lanes); }
-__device__ __forceinline__ int bounded(int position, int tokens) {
-  return static_cast<unsigned int>(position) < static_cast<unsigned int>(tokens) ? position : 0;
+/// How the rows without a token are dealt out to clearing workgroups: `rows` of them together, or a row in `parts`.
+struct clear_plan {
+  int rows;
+  int parts;
+  long long groups;
+};
+
+constexpr int clear_rows = gradient_threads;  ///< most rows per clearing workgroup
+
+/// Stores that go past the caches (`stream`): pieces of 8 KB, so that what the workgroups write at one time is close to one stretch of memory
+/// (131 072 rows of 8 KB, the whole pass: 186 us; pieces of 4 KB, half of whose time is the search for their rows, 292, of 16 KB 211, of 128
+/// KB 219).  Stores that the L2 gathers: 32 KB (50 021 rows of 4 004 bytes: 63 us; 8 KB 68, 16 and 64 KB 64).  More where the grid would
+/// not hold them.
+inline clear_plan clear_plan_for(int rows, std::size_t row_bytes, bool stream) {
+  clear_plan p;
+  for (std::size_t piece = stream ? 8192 : 32768;; piece *= 2) {
+    p.rows = row_bytes >= piece ? 1 : piece / row_bytes > clear_rows ? clear_rows : static_cast<int>(piece / row_bytes);
+    p.parts = static_cast<int>((row_bytes * p.rows + piece - 1) / piece);
+    p.groups = (static_cast<long long>(rows) + p.rows - 1) / p.rows * p.parts;
+    if (p.groups <= 3 << 22 || p.rows == clear_rows) return p;
+  }
 }
 
-/**
- * Every row of grad is written, rows without tokens with zeros.  One wavefront per (tile, slab); 64 tokens' keys and positions are loaded
- * at a time, one per lane, and become scalars as the wavefront walks over them with U gradient rows in flight.
- */
-template <int V, int U, bool STREAM, typename type_t, typename out_t>
-__global__ void __launch_bounds__(gradient_threads)
-gradient_overwrite(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows,
-                   const type_t* __restrict__ from, const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad,
-                   const std::size_t grad_pitch, const int tiles, const int items, const int slabs, tile_record* __restrict__ records,
-                   float* __restrict__ heads, float* __restrict__ tails) {
-  const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * gradient_waves + static_cast<int>(threadIdx.x) / wave::size);
-  const int tile = unit / slabs;
-  if (tile >= tiles) return;
-  const int part = unit - tile * slabs;
-  const lane_columns<V> cols(part, dim);
-  const long long total = static_cast<long long>(tokens) + rows;
-  const long long d0 = static_cast<long long>(tile) * items;
-  const long long d1 = d0 + items < total ? d0 + items : total;
-  int y = __builtin_amdgcn_readfirstlane(tokens_before(keys, tokens, d0));
-  int row = d0 > y ? static_cast<int>(d0 - y) : 0;
-  bool open = false;  // the row was begun by an earlier tile, and is cut here
-  if (y > 0 && row < rows && keys[y - 1] == row) {
-    const int behind = same_key<false>(keys, tokens, y, row);
-    open = same_key<true>(keys, tokens, y, row) + behind >= whole_row;
-    if (!open) {  // all of it, end included, is the earlier tile's
-      y += behind;
-      ++row;
-    }
+/// Zeros into those of the rows of clearing workgroup `group` that have no token.
+template <bool STREAM, typename out_t>
+__device__ __forceinline__ void clear_empty(const int* __restrict__ keys, int tokens, int rows, const clear_plan& plan, unsigned int group, int dim,
+                                            out_t* __restrict__ grad, std::size_t grad_pitch) {
+  __shared__ int s_range[2];
+  __shared__ int s_has[clear_rows];
+  const int tid = threadIdx.x;
+  const unsigned int place = group / plan.parts, part = group - place * plan.parts;
+  const int begin = static_cast<int>(place) * plan.rows;
+  const int count = rows - begin < plan.rows ? rows - begin : plan.rows, end = begin + count;
+  s_has[tid] = 0;
+  const int w = __builtin_amdgcn_readfirstlane(tid / wave::size);
+  if (w < 2) {
+    const int at = keys_below(keys, tokens, w == 0 ? begin : end);
+    if (wave::lane() == 0) s_range[w] = at;
   }
-  int begun = y;      // the row's first token here
-  int head_row = -1;
-  float acc[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-
-  const auto finish = [&]() {  // the row's end
-    if (open) {
-      head_row = row;
-      cols.store(heads + static_cast<std::size_t>(tile) * dim, acc);
-      open = false;
-    } else {
-      float v[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = scale * acc[k];
-      cols.template store<STREAM>(grad + static_cast<std::size_t>(row) * grad_pitch, v);
+  __syncthreads();
+  const int lo = s_range[0], hi = s_range[1];
+  if (count == 1) {
+    if (hi > lo) return;
+  } else if (hi - lo <= 4 * gradient_threads) {
+    for (int j = lo + tid; j < hi; j += gradient_threads) {
+      const unsigned int row = static_cast<unsigned int>(keys[j] - begin);
+      if (row < static_cast<unsigned int>(count)) s_has[row] = 1;
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-    ++row;
-  };
-  const auto clear_below = [&](int to) {  // rows without tokens
+  } else if (tid < count) {  // rows of many tokens: each is searched for
+    int l = lo, h = hi;
+    while (l < h) {
+      const int m = l + (h - l) / 2;
+      if (keys[m] < begin + tid) l = m + 1;
+      else h = m;
+    }
+    s_has[tid] = l < hi && keys[l] == begin + tid;
+  }
+  __syncthreads();
+  const auto fill = [&](auto v_tag) {
+    constexpr int V = decltype(v_tag)::value;
+    const unsigned int packets = (dim + V - 1) / V, all = packets * count;  // (parts > 1: one row)
+    const unsigned int per_part = (packets + plan.parts - 1) / plan.parts;
+    const unsigned int first = plan.parts > 1 ? part * per_part : 0, last = plan.parts > 1 && first + per_part < all ? first + per_part : all;
     const float zero[V] = {};
-    for (; row < to; ++row) cols.template store<STREAM>(grad + static_cast<std::size_t>(row) * grad_pitch, zero);
+    for (unsigned int i = first + tid; i < last; i += gradient_threads) {
+      const unsigned int row = i / packets;
+      const int own = static_cast<int>(i - row * packets) * V;
+      if (!s_has[row]) elements::store<V, STREAM>(grad + static_cast<std::size_t>(begin + row) * grad_pitch + (own + V <= dim ? own : dim - V), zero);
+    }
   };
-  const auto consume = [&](int key, int position, int count) {  // tokens y .. y + count, a lane each
-    for (int i = 0; i < count; i += U) {
-      elements::packet_t<type_t, V> packet[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = i + u < count ? i + u : count - 1;
-        packet[u] = elements::load<V>(from + static_cast<std::size_t>(__builtin_amdgcn_readlane(position, at)) * from_pitch + cols.at);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u < count) {
-          const int k = __builtin_amdgcn_readlane(key, i + u);
-          if (row < k) {
-            finish();
-            clear_below(k);
-            begun = y + i + u;
-          }
-#pragma unroll
-          for (int c = 0; c < V; ++c) acc[c] += static_cast<float>(packet[u][c]);
-        }
-      }
-    }
-    y += count;
-  };
-
-  int next_key = rows;  // of the token behind the tile's
-  for (;;) {
-    const int j = y + wave::lane();
-    int key = rows, position = 0;
-    if (j < tokens) {
-      key = keys[j];
-      position = bounded(positions[j], tokens);
-    }
-    const int count = leading(__ballot(is_row(key, rows) && static_cast<long long>(j) + key < d1));
-    consume(key, position, count);
-    if (count < wave::size) {
-      next_key = __builtin_amdgcn_readlane(key, count);
-      break;
-    }
-  }
-  // the rows that end in what is left of the tile (tokens without a row lie behind all of them)
-  const int row1 = d1 - y < rows ? static_cast<int>(d1 - y) : rows;
-  if (row < row1) {
-    finish();
-    clear_below(row1);
-    begun = y;
-  }
-  bool unfinished = open || y > begun;
-  if (unfinished && !open) {
-    const int behind = next_key == row ? same_key<false>(keys, tokens, y, row) : 0;
-    if (y - begun + behind < whole_row && row < rows) {  // a short row is finished here
-      const int j = y + wave::lane();
-      consume(row, j < tokens ? bounded(positions[j], tokens) : 0, behind);
-      finish();
-      unfinished = false;
-    }
-  }
-  if (unfinished) cols.store(tails + static_cast<std::size_t>(tile) * dim, acc);
-  if (part == 0 && wave::lane() == 0) records[tile] = tile_record{head_row, unfinished ? row : -1};
+  if (dim >= elements::per_access<out_t>) fill(std::integral_constant<int, elements::per_access<out_t>>{});
+  else fill(std::integral_constant<int, 1>{});
 }
 
 /**
- * Rows with tokens are added to.  Tiles of `items` tokens; otherwise as above.  What a row held is read together with the gradient
- * row of its last token, so that the two latencies are one.
+ * One wavefront per (tile, slab); 64 tokens' keys and positions are loaded at a time, one per lane, and become scalars as the wavefront
+ * walks over them with U gradient rows in flight.  ADD: rows with tokens are added to; what a row held is read together with the gradient
+ * row of its last token, so that the two latencies are one.  Otherwise rows with tokens are written, and the workgroups behind the tiles'
+ * write zeros into the others, in the order of memory: rows cleared from within the tiles, as they came in the list, left the chip at 5.2
+ * TB/s (8 192 tokens, 131 072 rows of 8 KB: 203 us, now 172, 6.6 TB/s).
+ * 8 wavefronts per SIMD are asked for: scalar registers would allow 7 otherwise (131 072 tokens x 4 096 bf16 into float, whole pass: 670
+ * us, 632 with 8: 5.1 TB/s of reads and writes together, where a copy of 4 GiB reaches 4.7).
  */
-template <int V, int U, typename type_t, typename out_t>
-__global__ void __launch_bounds__(gradient_threads)
-gradient_add(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows, const type_t* __restrict__ from,
-             const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad, const std::size_t grad_pitch,
-             const int tiles, const int items, const int slabs, tile_record* __restrict__ records, float* __restrict__ heads,
-             float* __restrict__ tails) {
+template <bool ADD, int V, int U, bool STREAM, typename type_t, typename out_t>
+__global__ void __launch_bounds__(gradient_threads, ADD ? 1 : 8)
+gradient(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows, const type_t* __restrict__ from,
+         const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad, const std::size_t grad_pitch, const int tiles,
+         const int items, const int slabs, const unsigned int tile_groups, const clear_plan clear, tile_record* __restrict__ records,
+         float* __restrict__ heads, float* __restrict__ tails) {
+  if constexpr (!ADD) {
+    if (blockIdx.x >= tile_groups) {
+      clear_empty<STREAM>(keys, tokens, rows, clear, blockIdx.x - tile_groups, dim, grad, grad_pitch);
+      return;
+    }
+  }
   const int unit = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * gradient_waves + static_cast<int>(threadIdx.x) / wave::size);
   const int tile = unit / slabs;
   if (tile >= tiles) return;
@@ -363,7 +325,7 @@ gradient_add(const int* __restrict__ keys, const int* __restrict__ positions, co
       for (int u = 0; u < U; ++u) {
         const int at = i + u < count ? i + u : count - 1;
         packet[u] = elements::load<V>(from + static_cast<std::size_t>(__builtin_amdgcn_readlane(position, at)) * from_pitch + cols.at);
-        if ((last >> at) & 1ull) old[u] = elements::load<V>(grad + static_cast<std::size_t>(__builtin_amdgcn_readlane(key, at)) * grad_pitch + cols.at);
+        if (ADD && ((last >> at) & 1ull)) old[u] = elements::load<V>(grad + static_cast<std::size_t>(__builtin_amdgcn_readlane(key, at)) * grad_pitch + cols.at);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -379,8 +341,8 @@ gradient_add(const int* __restrict__ keys, const int* __restrict__ positions, co
             } else {
               float v[V];
 #pragma unroll
-              for (int c = 0; c < V; ++c) v[c] = __builtin_fmaf(scale, acc[c], static_cast<float>(old[u][c]));
-              cols.store(grad + static_cast<std::size_t>(k) * grad_pitch, v);
+              for (int c = 0; c < V; ++c) v[c] = ADD ? __builtin_fmaf(scale, acc[c], static_cast<float>(old[u][c])) : scale * acc[c];
+              cols.template store<STREAM>(grad + static_cast<std::size_t>(k) * grad_pitch, v);
             }
 #pragma unroll
             for (int c = 0; c < V; ++c) acc[c] = 0.0f;
@@ -425,13 +387,13 @@ constexpr int small_waves = small_threads / wave::size;
 static_assert(small_tokens <= small_waves * wave::size, "a token per lane");
 
 /**
- * gradient_add for few tokens, in one launch: a workgroup adds all tokens of 64 columns, a sixteenth of them per wavefront, and rows
+ * gradient<ADD> for few tokens, in one launch: a workgroup adds all tokens of 64 columns, a sixteenth of them per wavefront, and rows
  * that several wavefronts hold are joined in LDS.  One column per lane: a row of the gradient is spread over as many CUs as there are
  * slabs (1 024 columns: 16), which few tokens leave idle otherwise.
  */
 template <int U, typename type_t, typename out_t>
 __global__ void __launch_bounds__(small_threads)
-gradient_add_small(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows,
+add_small(const int* __restrict__ keys, const int* __restrict__ positions, const int tokens, const int rows,
                    const type_t* __restrict__ from, const std::size_t from_pitch, const int dim, const float scale, out_t* __restrict__ grad,
                    const std::size_t grad_pitch) {
   __shared__ float s_tail[small_waves][wave::size];
@@ -502,13 +464,15 @@ constexpr int join_waves = join_threads / wave::size;
 
 /**
  * The rows that more than one tile holds: sum of the tails of the tiles before, in a fixed order, and the finishing tile's head.
- * A workgroup covers 256 columns and every gridDim.y-th tile; its wavefronts share a row's tails out.
+ * A workgroup covers 128 columns and every gridDim.y-th tile; its wavefronts share a row's tails out.  One CU's reads bound it (a row
+ * of 10 000 of 20 011 tokens leaves 590 tails of 1 001 columns: 16 us at 256 columns per workgroup, 12 at 128, 10 at 64, where the
+ * many short joins of 131 072 x 4 096 take 4 us more).
  */
 template <bool ADD, typename out_t>
 __global__ void __launch_bounds__(join_threads)
 join(const tile_record* __restrict__ records, const float* __restrict__ heads, const float* __restrict__ tails, const int tiles, const int dim,
      const float scale, out_t* __restrict__ grad, const std::size_t grad_pitch) {
-  constexpr int C = 4;  // columns per lane
+  constexpr int C = 2;  // columns per lane
   constexpr int U = 8;
   __shared__ float s_sum[join_waves][C][wave::size];
   const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / wave::size);
@@ -544,7 +508,7 @@ join(const tile_record* __restrict__ records, const float* __restrict__ heads, c
         run += n;
         if (n < wave::size) break;
       }
-      float sum[C] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float sum[C] = {};
       for (int b = tile - run + w; b < tile; b += join_waves * U) {
         float v[U][C];
 #pragma unroll
@@ -582,34 +546,31 @@ int launch_gradient(hipStream_t stream, const int* keys, const int* positions, i
                     int dim, float scale, bool add, out_t* grad, std::size_t grad_pitch, void* workspace) {
   if (rows == 0 || dim == 0 || (tokens == 0 && add)) return 0;
   if (add && tokens <= small_tokens) {
-    gradient_add_small<16, type_t, out_t><<<(dim + wave::size - 1) / wave::size, small_threads, 0, stream>>>(keys, positions, tokens, rows, from,
+    add_small<16, type_t, out_t><<<(dim + wave::size - 1) / wave::size, small_threads, 0, stream>>>(keys, positions, tokens, rows, from,
                                                                                                         from_pitch, dim, scale, grad, grad_pitch);
     return static_cast<int>(hipGetLastError());
   }
-  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, rows, dim, add);
+  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, dim);
   auto* const records = static_cast<tile_record*>(workspace);
   float* const heads = reinterpret_cast<float*>(static_cast<char*>(workspace) + gradient_records_bytes(p.tiles));
   float* const tails = heads + static_cast<std::size_t>(p.tiles) * dim;
-  const unsigned int grid = (static_cast<unsigned int>(p.tiles) * p.slabs + gradient_waves - 1) / gradient_waves;
-  const int column_groups = (dim + 255) / 256;
+  const unsigned int tile_groups = (static_cast<unsigned int>(p.tiles) * p.slabs + gradient_waves - 1) / gradient_waves;
+  const int column_groups = (dim + 127) / 128;
   const int most = 2048 / column_groups > 1 ? 2048 / column_groups : 1;
   const dim3 join_grid(column_groups, p.tiles < most ? p.tiles : most);
   const bool whole_lines = (reinterpret_cast<std::uintptr_t>(grad) | (grad_pitch * sizeof(out_t)) | (dim * sizeof(out_t))) % 128 == 0;
+  const clear_plan clear = clear_plan_for(rows, dim * sizeof(out_t), whole_lines);
   const auto run = [&](auto v_tag, auto add_tag) {
     constexpr int V = decltype(v_tag)::value;
     constexpr bool ADD = decltype(add_tag)::value;
-    if constexpr (ADD) {
-      gradient_add<V, 4, type_t, out_t><<<grid, gradient_threads, 0, stream>>>(keys, positions, tokens, rows, from, from_pitch, dim, scale, grad,
-                                                                              grad_pitch, p.tiles, p.items, p.slabs, records, heads, tails);
-    } else {
-      constexpr int U = V * sizeof(type_t) > 8 ? 8 : 16;  // 8 to 16 KB of a wavefront's loads in flight
-      const auto overwrite = [&](auto stream_tag) {
-        gradient_overwrite<V, U, decltype(stream_tag)::value, type_t, out_t><<<grid, gradient_threads, 0, stream>>>(
-            keys, positions, tokens, rows, from, from_pitch, dim, scale, grad, grad_pitch, p.tiles, p.items, p.slabs, records, heads, tails);
-      };
-      if (whole_lines) overwrite(std::true_type{});
-      else overwrite(std::false_type{});
-    }
+    constexpr int U = ADD ? 4 : V * sizeof(type_t) > 8 ? 8 : 16;  // 8 to 16 KB of a wavefront's loads in flight
+    const auto launch = [&](auto stream_tag) {
+      const unsigned int grid = tile_groups + (ADD ? 0u : static_cast<unsigned int>(clear.groups));
+      gradient<ADD, V, U, decltype(stream_tag)::value, type_t, out_t><<<grid, gradient_threads, 0, stream>>>(
+          keys, positions, tokens, rows, from, from_pitch, dim, scale, grad, grad_pitch, p.tiles, p.items, p.slabs, tile_groups, clear, records, heads, tails);
+    };
+    if (!ADD && whole_lines) launch(std::bool_constant<!ADD && (V > 1)>{});  // (whole lines are wider than an access)
+    else launch(std::false_type{});
     if (p.tiles > 1 && tokens >= whole_row)
       join<ADD, out_t><<<join_grid, join_threads, 0, stream>>>(records, heads, tails, p.tiles, dim, scale, grad, grad_pitch);
   };
