@@ -31,6 +31,7 @@ constexpr int lookup_threads = 256;
  * A row is cut into `packets` = ceil(dim / V) packets of V values, the last one shifted back to end with the row (its overlap is
  * written twice, with the same values): any width and alignment moves in 16-byte accesses.  Packets of all rows are numbered through
  * and each thread takes U of them, a workgroup's width apart: consecutive lanes touch consecutive packets whatever the width.
+ * HBM bounds it: 65 536 of 131 072 rows of 2 048 floats in 127 us, 5.9 TB/s; 16 tokens take 2.4 us, a launch.
  */
 template <int V, int U, bool STREAM, typename type_t, typename id_t>
 __global__ void __launch_bounds__(lookup_threads)
@@ -92,6 +93,9 @@ int launch_lookup(hipStream_t stream, const type_t* table, std::size_t table_pit
   };
   using one = std::integral_constant<int, 1>;
   using width = std::integral_constant<int, V>;
+  // Four packets per thread where that still fills the chip (bf16, dim 4 096: 512 tokens 3.4 us with one, 4.2 with four; 2 048: 6.6, 6.1;
+  // 16 384: 48.5, 41.0).  Stores of whole lines go past the caches (65 536 x 2 048 float: 160 us, 198 through them); others are left to the
+  // L2 to gather.
   const bool whole_lines = (reinterpret_cast<std::uintptr_t>(out) | (out_pitch * sizeof(type_t)) | (dim * sizeof(type_t))) % 128 == 0;
   const bool many = static_cast<unsigned long long>(tokens) * dim >= 512ull * lookup_threads * 4 * V;
   if (dim < V) return run(one{}, one{}, std::false_type{});
@@ -132,7 +136,9 @@ struct tile_record {
   int tail_row;
 };
 
-constexpr int small_tokens = 1024;  ///< most tokens of add_small
+/// One launch instead of two is 4 us of the host's time; its own grows with the tokens (x 1 024 bf16 into float: 128 tokens 6.2 us, 7.8 with the
+/// join; 512: 12.2, 7.9; 1 024: 22.2, 8.4).
+constexpr int small_tokens = 640;  ///< most tokens of add_small
 
 /// Workspace: records[tiles], heads[tiles][dim], tails[tiles][dim] (float).
 inline std::size_t gradient_records_bytes(int tiles) { return (static_cast<std::size_t>(tiles) * sizeof(tile_record) + 255) & ~static_cast<std::size_t>(255); }
@@ -465,7 +471,7 @@ constexpr int join_waves = join_threads / wave::size;
 /**
  * The rows that more than one tile holds: sum of the tails of the tiles before, in a fixed order, and the finishing tile's head.
  * A workgroup covers 128 columns and every gridDim.y-th tile; its wavefronts share a row's tails out.  One CU's reads bound it (a row
- * of 10 000 of 20 011 tokens leaves 590 tails of 1 001 columns: 16 us at 256 columns per workgroup, 12 at 128, 10 at 64, where the
+ * of 10 000 of 20 011 tokens leaves 590 tails of 1 001 columns: 16 us at 256 columns per workgroup, 13 at 128, 11 at 64, where the
  * many short joins of 131 072 x 4 096 take 4 us more).
  */
 template <bool ADD, typename out_t>

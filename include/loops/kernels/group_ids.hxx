@@ -15,6 +15,10 @@
  * A wavefront ranks 64 items at a time without atomics: one ballot per digit bit leaves each lane the mask of the lanes with its digit;
  * the rank is the number of mask bits below the lane and the last of them advances the wavefront's counter in LDS.  Items are taken in
  * order, so equal ids keep the order of their positions and the result is the same in every run.
+ *
+ * Few items are a matter of launches and of the latency of their dependent steps: 2 048 positions take 3.7 us by RANK (7.5 by one pass of
+ * the sort, 14.2 by two), 8 192 8.9 (8.3, 15.4), 16 384 26 (8.4, 16).  524 288 positions of 9 bits take 16 us in two launches, 131 072 of 18 bits
+ * 25 in four; more or fewer spans (64, 256) and holding the items in registers between counting and placing changed neither.
  */
 #pragma once
 

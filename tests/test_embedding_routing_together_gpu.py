@@ -170,6 +170,37 @@ def test_outputs_may_be_slices_and_inputs_shared():
     assert torch.equal(embedding.lookup(table, tokens), table[tokens.long()]) and torch.equal(embedding.lookup(other, tokens), other[tokens.long()])
 
 
+@pytest.mark.parametrize("dtype,dim,pitch", [(torch.float32, 4096, 4096), (torch.float32, 6176, 6176), (torch.float32, 6176, 6208), (torch.float32, 9001, 9001),
+                                             (torch.bfloat16, 64, 64), (torch.bfloat16, 64, 128), (torch.float16, 8200, 8200), (torch.bfloat16, 3, 3)])
+def test_rows_without_tokens_are_cleared(dtype, dim, pitch):
+    """Rows of a part of a clearing workgroup and of many to one, none or all of them without a token, the padding left as it was; whole numbers."""
+    from loops_amd import embedding
+    rng = np.random.default_rng(dim)
+    for rows, ids in [(1, [0]), (1, []), (700, []), (700, list(range(700))), (700, [0] * 70 + [699]), (701, [350] * 1500 + [351, 353, 700]), (65, [1, 3, 64, 3])]:
+        tokens = torch.tensor(ids, dtype=torch.int64, device="cuda")
+        grad = _whole(rng, len(ids), dim, dtype=dtype).clamp_(0, 1)
+        buffer = torch.full((rows, pitch), 5.0, device="cuda", dtype=dtype if dim < 5000 else torch.float32)
+        embedding.gradient(embedding.group_tokens(tokens, rows), grad, out=buffer[:, :dim])
+        want = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, tokens.cpu(), grad.cpu().double())
+        assert torch.equal(buffer[:, :dim].cpu().double(), want.to(buffer.dtype).double()), (rows, len(ids))
+        assert (buffer[:, dim:] == 5).all()
+
+
+@pytest.mark.parametrize("n", [63, 64, 639, 640, 641, 1024, 1025])
+def test_adding_few_tokens_and_some_more(n):
+    """Both sides of the one-launch form, tokens of one row, of all different rows and of some without a row."""
+    from loops_amd import embedding
+    rng = np.random.default_rng(n)
+    for ids in (np.full(n, 17), np.arange(n) % 2000, np.where(np.arange(n) % 3 == 0, -1, 1999), np.sort(rng.integers(0, 30, n)), np.full(n, -1)):
+        for dim in (1, 77, 520):
+            grad, old = _whole(rng, n, dim, dtype=torch.bfloat16), _whole(rng, 2000, dim)
+            tokens = torch.from_numpy(ids).cuda()
+            got = embedding.gradient(embedding.group_tokens(tokens, 2000), grad, scale=0.5, out=old.clone(), accumulate=True)
+            keep = torch.from_numpy(ids >= 0)
+            want = old.cpu().double().index_add_(0, torch.from_numpy(ids)[keep], 0.5 * grad.cpu().double()[keep])
+            assert torch.equal(got.cpu().double(), want), dim
+
+
 def test_refusals():
     from loops_amd import LoopsError, embedding, routing
     table, tokens = torch.zeros(9, 8, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
