@@ -96,7 +96,10 @@ def launch(device: int, name: str, *args) -> None:
 @functools.lru_cache(maxsize=4096)
 def workspace_bytes(name: str, *args) -> int:
     size = C.c_size_t(0)
-    L.check(getattr(L.lib(), name)(*args, C.byref(size)), name)
+    try:
+        L.check(getattr(L.lib(), name)(*args, C.byref(size)), name)
+    except C.ArgumentError as e:
+        raise TypeError(f"{name}: {e}") from None
     return size.value
 
 

@@ -176,6 +176,11 @@ def test_python_refusals(call, error):
         call()
 
 
+def test_sizes_that_are_no_integers_are_refused():
+    with pytest.raises(TypeError):
+        embedding.workspace_bytes("loops_expert_counts_workspace", 10, 2, 6.5)
+
+
 def test_sizes_beyond_the_int_arguments_are_refused_and_not_cut():
     embedding.c_int("loops_group_tokens", BIG, 0)
     for bad in (BIG + 1, 2 ** 32 + 5, -2 ** 32 + 5):
