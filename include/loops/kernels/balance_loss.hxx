@@ -510,7 +510,7 @@ inline groups_t share_out(int tokens, long long work_per_token, long long least,
   groups_t g;
   g.per = static_cast<int>((tokens + groups - 1) / groups);
   if (g.per < 1) g.per = 1;
-  g.groups = (tokens + g.per - 1) / g.per;
+  g.groups = static_cast<int>((static_cast<long long>(tokens) + g.per - 1) / g.per);  // (per is 4 million near 2^31 tokens)
   if (g.groups < 1) g.groups = 1;
   return g;
 }
