@@ -10,6 +10,7 @@
  */
 #pragma once
 
+#include <climits>
 #include <cstddef>
 #include <cstdint>
 #include <type_traits>
@@ -23,6 +24,20 @@
 namespace loops {
 namespace kernels {
 namespace embedding {
+
+/// Columns of one launch: the kernels' column numbers and grids stay within 32 bits (the gradient's of 16 threads per column the closest).
+constexpr int max_columns = 1 << 27;
+
+/// f(at, cols) for the column ranges [at, at + cols) of a matrix, until one returns an error: all columns at once up to max_columns.
+template <typename F>
+int by_columns(int dim, F&& f) {
+  for (int at = 0;;) {
+    const int cols = dim - at < max_columns ? dim - at : max_columns;
+    const int err = f(at, cols);
+    if (err || dim - at == cols) return err;
+    at += cols;
+  }
+}
 
 // ---- lookup -------------------------------------------------------------------------------------------------------------------
 constexpr int lookup_threads = 256;
@@ -81,14 +96,14 @@ int launch_lookup(hipStream_t stream, const type_t* table, std::size_t table_pit
                   const group_ids::key_map& map, float scale, type_t* out, std::size_t out_pitch) {
   if (tokens == 0 || dim == 0) return 0;
   constexpr int V = elements::per_access<type_t>;
-  const auto run = [&](auto v_tag, auto u_tag, auto stream_tag) {
+  const auto run = [&](auto v_tag, auto u_tag, auto stream_tag, int at, int cols) {  // columns [at, at + cols)
     constexpr int W = decltype(v_tag)::value, U = decltype(u_tag)::value;
-    const int packets = (dim + W - 1) / W;
+    const int packets = (cols + W - 1) / W;
     const unsigned long long all = static_cast<unsigned long long>(tokens) * packets;
     const unsigned long long grid = (all + lookup_threads * U - 1) / (lookup_threads * U);
     if (grid * lookup_threads >= (1ull << 32)) return static_cast<int>(hipErrorInvalidValue);
     lookup<W, U, decltype(stream_tag)::value, type_t, id_t><<<static_cast<unsigned int>(grid), lookup_threads, 0, stream>>>(
-        table, table_pitch, ids, tokens, packets, dim, map, scale, out, out_pitch);
+        table + at, table_pitch, ids, tokens, packets, cols, map, scale, out + at, out_pitch);
     return static_cast<int>(hipGetLastError());
   };
   using one = std::integral_constant<int, 1>;
@@ -98,9 +113,12 @@ int launch_lookup(hipStream_t stream, const type_t* table, std::size_t table_pit
   // L2 to gather.
   const bool whole_lines = (reinterpret_cast<std::uintptr_t>(out) | (out_pitch * sizeof(type_t)) | (dim * sizeof(type_t))) % 128 == 0;
   const bool many = static_cast<unsigned long long>(tokens) * dim >= 512ull * lookup_threads * 4 * V;
-  if (dim < V) return run(one{}, one{}, std::false_type{});
-  if (!many) return run(width{}, one{}, std::false_type{});
-  return whole_lines ? run(width{}, std::integral_constant<int, 4>{}, std::true_type{}) : run(width{}, std::integral_constant<int, 4>{}, std::false_type{});
+  return by_columns(dim, [&](int at, int cols) {
+    if (cols < V) return run(one{}, one{}, std::false_type{}, at, cols);
+    if (!many) return run(width{}, one{}, std::false_type{}, at, cols);
+    return whole_lines ? run(width{}, std::integral_constant<int, 4>{}, std::true_type{}, at, cols)
+                       : run(width{}, std::integral_constant<int, 4>{}, std::false_type{}, at, cols);
+  });
 }
 
 // ---- gradient -----------------------------------------------------------------------------------------------------------------
@@ -123,7 +141,7 @@ inline gradient_plan gradient_plan_for(int width, int tokens, int dim) {
   gradient_plan p;
   p.slabs = (dim + wave::size * width - 1) / (wave::size * width);
   long long items = (static_cast<long long>(tokens) * p.slabs + 16383) / 16384;
-  items = items < 16 ? 16 : items;
+  items = items < 16 ? 16 : items > INT_MAX ? INT_MAX : items;
   p.items = static_cast<int>(items);
   p.tiles = static_cast<int>((tokens + items - 1) / items);
   return p;
@@ -145,8 +163,14 @@ inline std::size_t gradient_records_bytes(int tiles) { return (static_cast<std::
 template <typename type_t, typename out_t>
 std::size_t gradient_workspace_bytes(int tokens, int rows, int dim, bool add) {
   if (dim == 0 || rows == 0 || (add && tokens <= small_tokens)) return 0;
-  const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, dim);
-  return gradient_records_bytes(p.tiles) + 2 * static_cast<std::size_t>(p.tiles) * dim * sizeof(float);
+  std::size_t most = 0;  // column ranges follow each other in the same memory
+  by_columns(dim, [&](int, int cols) {
+    const gradient_plan p = gradient_plan_for(lane_width<type_t, out_t>, tokens, cols);
+    const std::size_t bytes = gradient_records_bytes(p.tiles) + 2 * static_cast<std::size_t>(p.tiles) * cols * sizeof(float);
+    most = bytes > most ? bytes : most;
+    return 0;
+  });
+  return most;
 }
 
 /// Ids and positions that group_ids did not write are not followed out of the arrays, whatever they are: positions are bounded, ids count
@@ -547,10 +571,10 @@ join(const tile_record* __restrict__ records, const float* __restrict__ heads, c
   }
 }
 
+/// One range of columns (at most max_columns).
 template <typename type_t, typename out_t>
-int launch_gradient(hipStream_t stream, const int* keys, const int* positions, int tokens, int rows, const type_t* from, std::size_t from_pitch,
-                    int dim, float scale, bool add, out_t* grad, std::size_t grad_pitch, void* workspace) {
-  if (rows == 0 || dim == 0 || (tokens == 0 && add)) return 0;
+int launch_gradient_columns(hipStream_t stream, const int* keys, const int* positions, int tokens, int rows, const type_t* from,
+                            std::size_t from_pitch, int dim, float scale, bool add, out_t* grad, std::size_t grad_pitch, void* workspace) {
   if (add && tokens <= small_tokens) {
     add_small<16, type_t, out_t><<<(dim + wave::size - 1) / wave::size, small_threads, 0, stream>>>(keys, positions, tokens, rows, from,
                                                                                                         from_pitch, dim, scale, grad, grad_pitch);
@@ -589,6 +613,16 @@ int launch_gradient(hipStream_t stream, const int* keys, const int* positions, i
     else run(std::integral_constant<int, V>{}, std::false_type{});
   }
   return static_cast<int>(hipGetLastError());
+}
+
+template <typename type_t, typename out_t>
+int launch_gradient(hipStream_t stream, const int* keys, const int* positions, int tokens, int rows, const type_t* from, std::size_t from_pitch,
+                    int dim, float scale, bool add, out_t* grad, std::size_t grad_pitch, void* workspace) {
+  if (rows == 0 || dim == 0 || (tokens == 0 && add)) return 0;
+  return by_columns(dim, [&](int at, int cols) {
+    return launch_gradient_columns<type_t, out_t>(stream, keys, positions, tokens, rows, from + at, from_pitch, cols, scale, add, grad + at, grad_pitch,
+                                                  workspace);
+  });
 }
 
 }  // namespace embedding

@@ -25,3 +25,20 @@ def test_workgroups_share_out_every_token(tokens):
     experts = 16
     assert _bytes("loops_expert_counts_workspace", tokens, 1, experts) == groups * experts * 4
     assert _bytes("loops_balance_loss_workspace", tokens, experts) == (groups * (2 * 64 + 1) + 1 + 1) * 4
+
+
+@pytest.mark.parametrize("grad_type,out_type,width", [(BF16, F32, 4), (F16, F16, 8), (F32, F32, 4)])
+@pytest.mark.parametrize("tokens", [1, 100, 5000])
+def test_gradient_workspace_of_the_widest_rows(grad_type, out_type, width, tokens):
+    """Rows are worked on 2^27 columns at a time: the workspace is that of as many columns, whatever the whole width, up to 2^31 - 1."""
+    columns = 2 ** 27
+    slabs = columns // (64 * width)
+    items = max(16, -(-tokens * slabs // 16384))
+    tiles = -(-tokens // items)
+    bytes_of = lambda dim: _bytes("loops_embedding_gradient_workspace", grad_type, out_type, tokens, 7, dim, 0)  # noqa: E731
+    want = -(-tiles * 8 // 256) * 256 + 2 * tiles * columns * 4
+    assert bytes_of(columns) == want
+    for dim in (columns + 1, columns + 100000, 2 ** 31 - 600, 2 ** 31 - 513, 2 ** 31 - 512, 2 ** 31 - 100, 2 ** 31 - 1):
+        # (the last range, narrower, may be cut into more tiles: by a tile's rounding at most)
+        assert want <= bytes_of(dim) <= 2 * want, dim
+    assert _bytes("loops_embedding_gradient_workspace", grad_type, out_type, 2 ** 30, 7, 2 ** 31 - 1, 0) > 0  # (more than any memory, and no overflow)

@@ -22,3 +22,48 @@ def test_counts_and_loss_of_the_most_tokens():
     bound = 2.0 ** -24 * 520
     assert abs(forward.probability.item() - 1.0) <= bound
     assert abs(forward.loss.item() - 0.5 * (tokens - 5) / tokens) <= 0.5 * 2 * bound
+
+
+def _whole(rows, cols, seed):
+    """Whole numbers in [-4, 4], half, made a row at a time."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    out = torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    for r in range(rows):
+        out[r] = torch.randint(-4, 5, (cols,), generator=g, dtype=torch.int8, device="cuda")
+    return out
+
+
+def _same(got, want):
+    """Equal, compared a piece at a time (a comparison of all of it makes a temporary as large)."""
+    assert got.shape == want.shape
+    for at in range(0, got.numel(), 2 ** 28):
+        assert torch.equal(got[at:at + 2 ** 28], want[at:at + 2 ** 28]), at
+
+
+def test_the_widest_rows():
+    """2^31 - 1 columns, and 2^28 + 5, which end in a range narrower than an access; whole numbers and a scale of 2: exact sums."""
+    from loops_amd import embedding
+    dim = 2 ** 31 - 1
+    table = _whole(2, dim, 1)
+    got = embedding.lookup(table, torch.tensor([1, 7], device="cuda"), scale=2.0)
+    _same(got[0], table[1] * 2)
+    assert not got[1].any()
+    del got
+    groups = embedding.group_tokens(torch.tensor([2, 2], device="cuda"), 3)
+    got = embedding.gradient(groups, table, scale=2.0)
+    assert not got[0].any() and not got[1].any()
+    _same(got[2], (table[0] + table[1]) * 2)
+    embedding.gradient(groups, table, scale=2.0, out=got, accumulate=True)  # in one launch per range
+    assert not got[0].any() and not got[1].any()
+    _same(got[2], (table[0] + table[1]) * 4)
+    del got, table
+    dim, tokens = 2 ** 28 + 5, 70  # (the row is cut into tiles and joined in the last, narrow range)
+    grad = _whole(tokens, dim, 2)
+    groups = embedding.group_tokens(torch.ones(tokens, dtype=torch.int64, device="cuda"), 2)
+    got = embedding.gradient(groups, grad)
+    assert not got[0].any()
+    want = torch.zeros(dim, dtype=torch.float16, device="cuda")  # (sums of 70 numbers up to 4 are exact in half)
+    for t in range(tokens):
+        want += grad[t]
+    _same(got[1], want)
