@@ -25,6 +25,8 @@ namespace loops {
 namespace kernels {
 namespace embedding {
 
+/// Threads that one dimension of a grid holds.
+constexpr unsigned long long max_launch_threads = (1ull << 32) - 1;
 /// Columns of one launch: the kernels' column numbers and grids stay within 32 bits (the gradient's of 16 threads per column the closest).
 constexpr int max_columns = 1 << 27;
 
@@ -96,15 +98,20 @@ int launch_lookup(hipStream_t stream, const type_t* table, std::size_t table_pit
                   const group_ids::key_map& map, float scale, type_t* out, std::size_t out_pitch) {
   if (tokens == 0 || dim == 0) return 0;
   constexpr int V = elements::per_access<type_t>;
-  const auto run = [&](auto v_tag, auto u_tag, auto stream_tag, int at, int cols) {  // columns [at, at + cols)
+  // columns [at, at + cols) of all tokens, in as few launches as hold them (one but for some 2^32 packets)
+  const auto run = [&](auto v_tag, auto u_tag, auto stream_tag, int at, int cols) {
     constexpr int W = decltype(v_tag)::value, U = decltype(u_tag)::value;
     const int packets = (cols + W - 1) / W;
-    const unsigned long long all = static_cast<unsigned long long>(tokens) * packets;
-    const unsigned long long grid = (all + lookup_threads * U - 1) / (lookup_threads * U);
-    if (grid * lookup_threads >= (1ull << 32)) return static_cast<int>(hipErrorInvalidValue);
-    lookup<W, U, decltype(stream_tag)::value, type_t, id_t><<<static_cast<unsigned int>(grid), lookup_threads, 0, stream>>>(
-        table + at, table_pitch, ids, tokens, packets, cols, map, scale, out + at, out_pitch);
-    return static_cast<int>(hipGetLastError());
+    const long long most = static_cast<long long>(max_launch_threads / lookup_threads) * (lookup_threads * U) / packets;
+    for (long long t = 0; t < tokens; t += most) {
+      const int count = static_cast<int>(tokens - t < most ? tokens - t : most);
+      const unsigned long long all = static_cast<unsigned long long>(count) * packets;
+      const unsigned int grid = static_cast<unsigned int>((all + lookup_threads * U - 1) / (lookup_threads * U));
+      lookup<W, U, decltype(stream_tag)::value, type_t, id_t><<<grid, lookup_threads, 0, stream>>>(
+          table + at, table_pitch, ids + t, count, packets, cols, map, scale, out + static_cast<std::size_t>(t) * out_pitch + at, out_pitch);
+      if (const hipError_t err = hipGetLastError()) return static_cast<int>(err);
+    }
+    return 0;
   };
   using one = std::integral_constant<int, 1>;
   using width = std::integral_constant<int, V>;

@@ -67,3 +67,15 @@ def test_the_widest_rows():
     for t in range(tokens):
         want += grad[t]
     _same(got[1], want)
+
+
+def test_more_narrow_lookups_than_a_launch_holds():
+    """2^30 tokens of rows of 4 halves, moved one by one: more than 2^32 threads."""
+    from loops_amd import embedding
+    rows, dim, tokens = 1000, 4, 2 ** 30 + 77
+    table = _whole(rows, dim, 3)
+    ids = torch.arange(tokens, dtype=torch.int32, device="cuda").remainder_(rows + 3)  # three in 1 003 lie outside
+    got = embedding.lookup(table, ids, scale=0.5)
+    padded = torch.cat([table * 0.5, torch.zeros(3, dim, dtype=torch.float16, device="cuda")])
+    for at in range(0, tokens, 2 ** 26):
+        assert torch.equal(got[at:at + 2 ** 26], padded[ids[at:at + 2 ** 26].long()]), at
