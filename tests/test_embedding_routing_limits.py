@@ -42,3 +42,15 @@ def test_gradient_workspace_of_the_widest_rows(grad_type, out_type, width, token
         # (the last range, narrower, may be cut into more tiles: by a tile's rounding at most)
         assert want <= bytes_of(dim) <= 2 * want, dim
     assert _bytes("loops_embedding_gradient_workspace", grad_type, out_type, 2 ** 30, 7, 2 ** 31 - 1, 0) > 0  # (more than any memory, and no overflow)
+
+
+A, B, D, G, H = (1 << 40, 2 << 40, 3 << 40, 4 << 40, 5 << 40)  # addresses far apart, never read
+
+
+@pytest.mark.parametrize("off", [1, 4, 8, 12])
+def test_workspaces_that_are_not_16_byte_aligned_are_refused(off):
+    lib, size = _lib.lib(), 1 << 40
+    assert lib.loops_group_tokens(I64, 9000, A, 100, 0, -1, B, D, G + off, size, None) == BADARG
+    assert lib.loops_embedding_gradient(BF16, F32, 2000, A, B, 30, 16, D, 16, 1.0, 0, G, 16, H + off, size, None) == BADARG
+    assert lib.loops_expert_counts(I64, 100000, 4, A, None, 16, B, G + off, size, None) == BADARG
+    assert lib.loops_balance_loss(F32, I64, 100000, 16, 4, A, 16, B, None, 1.0, D, D + 64, D + 256, D + 512, G + off, size, None) == BADARG
