@@ -8,6 +8,10 @@ rows of every id.  Tables, gradients and results are float32, float16 or bfloat1
 Calls are asynchronous on the current stream of the tensors' device and may be captured into a graph; there is no CPU path.  Arguments
 of a wrong type raise TypeError, of a wrong shape or layout ValueError; what the library itself refuses (an output that overlaps an
 input, sizes beyond its range) LoopsError.
+
+Autograd records none of these calls; the gradients are calls of their own.  A table that requires a gradient is therefore refused
+(ValueError) where autograd records, as is any ``out`` that does: call under ``torch.no_grad()``, on ``table.detach()``, or from the forward
+and backward of a ``torch.autograd.Function``, where it does not.
 """
 from __future__ import annotations
 
@@ -61,6 +65,12 @@ def pitch_of(t: torch.Tensor, what: str) -> int:
     if (step != 1 and cols != 1) or pitch < cols:
         raise ValueError(f"{what}: columns must be adjacent and rows must not overlap")
     return pitch
+
+
+def not_recorded(what: str) -> None:
+    """Refuses a tensor that requires a gradient where autograd would record an operation on it: the gradient would be lost without an error."""
+    if torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which this call does not record: use torch.no_grad(), {what}.detach() or an autograd.Function")
 
 
 INT_MAX = 2 ** 31 - 1
@@ -118,6 +128,10 @@ def lookup(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, first_
     ``table``: [rows, dim], columns adjacent, any distance between rows.  ``tokens``: any shape, contiguous.  ``out``:
     [*tokens.shape, dim] contiguous (or [tokens, dim] with any distance between rows), of the table's type; made when not given."""
     value, index = value_type(table, "table"), index_type(tokens, "tokens")
+    if table.requires_grad:
+        not_recorded("table")
+    if out is not None and out.requires_grad:
+        not_recorded("out")
     pitch = pitch_of(table, "table")
     if not tokens.is_contiguous():
         raise ValueError("tokens must be contiguous")
@@ -175,6 +189,8 @@ def gradient(groups: TokenGroups, grad: torch.Tensor, scale: float = 1.0, dtype:
     float32 (``dtype`` when it is made here).  ``accumulate``: add to what ``out`` holds in the rows that have tokens and leave the
     others.  Sums are held in float32 and rounded once; their order is fixed."""
     value = value_type(grad, "grad")
+    if out is not None and out.requires_grad:
+        not_recorded("out")
     ids, positions, rows = groups
     n = ids.numel()
     if ids.dtype is not torch.int32 or positions.dtype is not torch.int32:

@@ -9,6 +9,9 @@ The order in which experts take their tokens is ``embedding.group_tokens(chosen,
 expert indices int32 or int64 (one outside [0, experts) is not counted).  Calls are asynchronous on the current stream of the tensors'
 device and may be captured into a graph; there is no CPU path.  Arguments of a wrong type raise TypeError, of a wrong shape or layout
 ValueError; what the library itself refuses (an output that overlaps an input, sizes beyond its range) LoopsError.
+
+Autograd records none of these calls: ``balance_loss`` refuses logits that require a gradient (ValueError) where it does record.  Call it
+under ``torch.no_grad()``, on ``logits.detach()``, or from a ``torch.autograd.Function`` whose backward calls ``balance_loss_backward``.
 """
 from __future__ import annotations
 
@@ -16,7 +19,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .embedding import c_int, index_type, launch, pitch_of, same_device, value_type, workspace
+from .embedding import c_int, index_type, launch, not_recorded, pitch_of, same_device, value_type, workspace
 
 
 def _mask(mask: Optional[torch.Tensor], tokens: int):
@@ -60,6 +63,8 @@ def balance_loss(logits: torch.Tensor, chosen: torch.Tensor, coefficient: float 
     """The balance loss of ``logits`` [tokens, experts] (any distance between rows) for the experts ``chosen`` [tokens, choices] (contiguous);
     ``mask`` [tokens]: the tokens that take part (all where it is None)."""
     value, index = value_type(logits, "logits"), index_type(chosen, "chosen")
+    if logits.requires_grad:
+        not_recorded("logits")
     pitch = pitch_of(logits, "logits")
     tokens, experts = logits.shape
     if chosen.dim() != 2 or chosen.shape[0] != tokens or not chosen.is_contiguous():
@@ -83,6 +88,8 @@ def balance_loss_backward(logits: torch.Tensor, forward: BalanceLoss, mask: Opti
     """Gradient of ``grad_loss * loss`` (a float32 scalar on the device; 1 where it is None) with respect to ``logits``, in their type: [tokens,
     experts].  ``logits`` and ``mask`` as in the forward call, ``forward`` what it returned."""
     value = value_type(logits, "logits")
+    if out is not None and out.requires_grad:
+        not_recorded("out")
     pitch = pitch_of(logits, "logits")
     tokens, experts = logits.shape
     if forward.counts.shape != (experts,):
