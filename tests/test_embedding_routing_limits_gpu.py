@@ -79,3 +79,61 @@ def test_more_narrow_lookups_than_a_launch_holds():
     padded = torch.cat([table * 0.5, torch.zeros(3, dim, dtype=torch.float16, device="cuda")])
     for at in range(0, tokens, 2 ** 26):
         assert torch.equal(got[at:at + 2 ** 26], padded[ids[at:at + 2 ** 26].long()]), at
+
+
+def test_balance_loss_and_gradient_beyond_32_bit_offsets():
+    """2 100 003 x 1 024 logits (2.15e9 of them), whole rows at both ends and between against float64.
+
+    Bounds as in test_routing_gpu.py: e = 2^-24, a probability is off by P = (2 D + E + 8) e relative, their mean over n tokens by (n + 3) e more (the
+    sums are of at most n terms, all positive), the loss by (n + E + 8) e instead; the gradient by (2 P + (E + 16) e) s p (f + d) and half a step of
+    bfloat16, 2^-8, of its value.  n e would be 1/8 here; no sum adds more than 1 024 terms after each other (4 102 tokens per workgroup are 257 rows per
+    wavefront, then 16 wavefronts, then 512 workgroups), which stand in n's place.  Float32's least normal number, 2^-126, for each exponential."""
+    from loops_amd import routing
+    tokens, experts, choices, e = 2100003, 1024, 2, 2.0 ** -24
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    logits = torch.empty(tokens, experts, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    chosen = torch.randint(-1, experts, (tokens, choices), generator=g, dtype=torch.int32, device="cuda")
+    mask = torch.rand(tokens, generator=g, device="cuda") < 0.9
+    forward = routing.balance_loss(logits, chosen, coefficient=1.0, mask=mask)
+    n = int(mask.sum())
+    kept = chosen[mask].reshape(-1).long()
+    counts = torch.bincount(kept[kept >= 0], minlength=experts)
+    total, distance = torch.zeros(experts, dtype=torch.float64, device="cuda"), 0.0
+    for at in range(0, tokens, 2 ** 17):
+        x = logits[at:at + 2 ** 17].double()
+        x -= x.amax(1, keepdim=True)
+        distance = max(distance, -x.min().item())
+        p = x.exp_()
+        p /= p.sum(1, keepdim=True)
+        total += (p * mask[at:at + 2 ** 17, None]).sum(0)
+    f, mean = counts.double() / (n * choices), total / n
+    loss = experts * (f * mean).sum().item()
+    rel = 1.01 * (2 * distance + experts + 8) * e
+    assert forward.tokens.item() == n and torch.equal(forward.counts.long(), counts)
+    assert ((forward.probability.double() - mean).abs() <= (rel + 1.01 * (1024 + 3) * e) * mean + 2.0 ** -126).all()
+    assert abs(forward.loss.item() - loss) <= (rel + 1.01 * (1024 + experts + 8) * e) * loss
+
+    grad = routing.balance_loss_backward(logits, forward, mask=mask, grad_loss=torch.full((), float(n), device="cuda"))
+    middle = 2 ** 31 // experts  # the row behind the last element that 31 bits number
+    at = torch.cat([torch.arange(300), torch.arange(middle - 300, middle + 300), torch.arange(tokens - 300, tokens),
+                    torch.randint(tokens, (3000,))]).cuda()
+    p = torch.softmax(logits[at].double(), 1) * mask[at, None]
+    d = (p * f).sum(1, keepdim=True)
+    want, size = experts * p * (f - d), experts * p * (f + d)
+    bound = size * (2 * rel + 1.01 * (experts + 16) * e) + 2.0 ** -8 * 1.01 * want.abs() + experts * 2.0 ** -126
+    assert ((grad[at].double() - want).abs() <= bound).all()
+    assert (grad[at][~mask[at]] == 0).all() and (grad[at][mask[at]] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("n", [131071, 131072, 131073, 262145, 1200008])
+@pytest.mark.parametrize("rows", [256, 131072])
+def test_group_tokens_in_spans_of_more_than_1024(n, rows):
+    """Up to 128 spans of 1 024 positions each; beyond that longer spans."""
+    from loops_amd import embedding
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n)
+    ids = torch.randint(-1, rows, (n,), generator=g, device="cuda")
+    got = embedding.group_tokens(ids, rows)
+    key, order = torch.sort(torch.where(ids < 0, rows, ids), stable=True)
+    assert torch.equal(got.ids.long(), key) and torch.equal(got.positions.long(), order)
