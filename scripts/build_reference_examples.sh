@@ -9,7 +9,7 @@ REF=${REF:-/root/reference}
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 OUT=$ROOT/build/examples
 mkdir -p "$OUT"
-FLAGS="--offload-arch=gfx950 -std=c++17 -O3 -x hip -DLOOPS_TARGET_GFX=0x950 -Wno-unused-result -I$ROOT/include -I$ROOT/third_party/cxxopts"
+FLAGS="--offload-arch=gfx950 -std=c++17 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -x hip -DLOOPS_TARGET_GFX=0x950 -Wno-unused-result -I$ROOT/include -I$ROOT/third_party/cxxopts"
 fail=0
 build() {  # src out extra-flags
   if /opt/rocm/bin/hipcc $FLAGS $3 "$1" -o "$2" > "$2.log" 2>&1; then echo "ok   $(basename $2)"; else echo "FAIL $(basename $2) (see $2.log)"; fail=1; fi

@@ -9,7 +9,7 @@ REF=${REF:-/root/reference}
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 OUT=$ROOT/build/unittests
 mkdir -p "$OUT"
-FLAGS="--offload-arch=gfx950 -std=c++17 -O2 -x hip -DLOOPS_TARGET_GFX=0x950 -Wno-unused-result -I$ROOT/include -I$ROOT/tests/stubs -I$REF/unittests"
+FLAGS="--offload-arch=gfx950 -std=c++17 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -x hip -DLOOPS_TARGET_GFX=0x950 -Wno-unused-result -I$ROOT/include -I$ROOT/tests/stubs -I$REF/unittests"
 fail=0
 JOBS=${JOBS:-$(nproc)}
 n=0

@@ -10,6 +10,13 @@ if ROOT not in sys.path:
 
 GOLDEN = os.path.join(ROOT, "tests", "golden")
 
+# the C++ tests call hipcc themselves: their device code is built as the library's is, without packed fp32 instructions
+from loops_amd._lib import DEVICE_FLAGS  # noqa: E402
+
+_flags = os.environ.get("HIPCC_COMPILE_FLAGS_APPEND", "")
+if DEVICE_FLAGS[-1] not in _flags.split():
+    os.environ["HIPCC_COMPILE_FLAGS_APPEND"] = " ".join([_flags, *DEVICE_FLAGS]).strip()
+
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with `-m gpu` on the GPU box)")

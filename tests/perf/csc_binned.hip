@@ -1,5 +1,5 @@
 // Harness of tests/perf/exp_csc_binned.py: the binned one-shot CSC product next to the atomic kernels.
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -DLOOPS_TARGET_GFX=0x950 -Iinclude tests/perf/csc_binned.hip -o build/variants/libcsc_binned.so
+// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC -DLOOPS_TARGET_GFX=0x950 -Iinclude tests/perf/csc_binned.hip -o build/variants/libcsc_binned.so
 #include <hip/hip_runtime.h>
 #include <loops/kernels/csc_spmv.hxx>
 using namespace loops;

@@ -8,7 +8,7 @@
 // M passes: pass p takes the items whose index lies in [p, p + 1) * table / M (execution-masked loads), and waits.
 // Workgroups start together and do equal work, so passes line up in time by themselves ("natural lockstep"); LOCK = 1
 // additionally picks the first pass from a shared clock (s_memrealtime / period).
-// Build: hipcc -O3 --offload-arch=gfx950 -shared -fPIC -o build/variants/libexp_phased.so tests/perf/exp_phased_gather.hip
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC -o build/variants/libexp_phased.so tests/perf/exp_phased_gather.hip
 #include <hip/hip_runtime.h>
 #include <cstddef>
 #include <cstdint>

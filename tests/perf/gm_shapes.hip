@@ -1,5 +1,5 @@
 // Harness of tests/perf/exp_group_mapped_shapes.py: group_mapped (heavy groups shared out) for several group sizes / tile shapes behind a C ABI.
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -DLOOPS_TARGET_GFX=0x950 -Iinclude tests/perf/gm_shapes.hip -o build/variants/libgm_shapes.so
+// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC -DLOOPS_TARGET_GFX=0x950 -Iinclude tests/perf/gm_shapes.hip -o build/variants/libgm_shapes.so
 #include <hip/hip_runtime.h>
 #include <loops/kernels/launch.hxx>
 #include <loops/kernels/group_mapped_spmv.hxx>

@@ -1,6 +1,6 @@
 // Harness of tests/perf/exp_thread_mapped_assisted.py: the tuned thread_mapped launch, the assisted kernel instantiated directly (fp32, fp64)
 // and the reference-shaped loop behind a C ABI.  Build (dev container, no GPU needed):
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -DLOOPS_TARGET_GFX=0x950 -Iinclude tests/perf/tm_assist.hip -o build/variants/libtm_assist.so
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -shared -fPIC -DLOOPS_TARGET_GFX=0x950 -Iinclude tests/perf/tm_assist.hip -o build/variants/libtm_assist.so
 #include <hip/hip_runtime.h>
 #include <loops/kernels/csr_spmv.hxx>
 #include <loops/kernels/launch.hxx>
