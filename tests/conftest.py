@@ -22,6 +22,18 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with `-m gpu` on the GPU box)")
 
 
+# What runs programs that only the reference's sources can be built into (scripts/build_reference_*.sh, oracle/Makefile)
+NEEDS_REFERENCE_PROGRAMS = ("test_examples_gpu.py", "test_reference_unittests_gpu.py", "test_ref_gpu_pin.py", "test_against_the_reference_kernel_on_this_gpu")
+
+
+def pytest_collection_modifyitems(items):
+    """Where those programs were never built, the tests that need them run last (and fail there, as before): a run with -x has then run all
+    others."""
+    built = (os.path.join(ROOT, *p) for p in (("build", "examples"), ("build", "unittests"), ("oracle", "_ref")))
+    if not all(os.path.isdir(p) for p in built):
+        items.sort(key=lambda item: any(name in item.nodeid for name in NEEDS_REFERENCE_PROGRAMS))
+
+
 # --------------------------------------------------------------------------------------------
 # The hermetic matrix battery: same shapes the reference's SpMV battery exercises
 # (unittests/test_spmv_battery.hxx:52-65: identity, diagonal, banded, block-diagonal, skewed,
