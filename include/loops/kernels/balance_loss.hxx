@@ -203,14 +203,14 @@ struct outputs {
 };
 
 namespace detail {
-/// Writes column e's outputs and returns its term of the loss.
+/// Writes column e's outputs and returns its term of the loss.  Factors of a whole result are products of double, rounded once.
 __device__ __forceinline__ float finish_column(int e, float sum, int count, int tokens, int experts, int choices, const outputs& out) {
   if (e >= experts) return 0.0f;
-  const float per_token = tokens > 0 ? 1.0f / static_cast<float>(tokens) : 0.0f;
-  const float probability = sum * per_token;
+  const double per_token = tokens > 0 ? 1.0 / tokens : 0.0;
+  const double probability = sum * per_token;
   out.counts[e] = count;
-  out.probability[e] = probability;
-  return static_cast<float>(count) * per_token / static_cast<float>(choices) * probability;
+  out.probability[e] = static_cast<float>(probability);
+  return static_cast<float>(count * per_token / choices * probability);
 }
 }  // namespace detail
 
@@ -301,7 +301,7 @@ forward(const type_t* __restrict__ logits, const std::size_t pitch, const id_t* 
     const float term = detail::finish_column(tid, total, tid < experts ? s_count[tid] : 0, s_tokens, experts, choices, out);
     const float loss = detail::block_sum(term, s_scratch);
     if (tid == 0) {
-      *out.loss = coefficient * static_cast<float>(experts) * loss;
+      *out.loss = static_cast<float>(static_cast<double>(coefficient) * experts * loss);
       *out.tokens = s_tokens;
     }
   } else {
@@ -404,7 +404,7 @@ finish_forward(const float* __restrict__ sums, const int* __restrict__ counts, c
       const float loss = detail::row_sum<wave::size>(
           lane < static_cast<int>(gridDim.x) ? __hip_atomic_load(parts + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f);
       if (lane == 0) {
-        *out.loss = coefficient * static_cast<float>(experts) * loss;
+        *out.loss = static_cast<float>(static_cast<double>(coefficient) * experts * loss);
         *out.tokens = s_tokens;
       }
     }
@@ -421,14 +421,14 @@ backward(const type_t* __restrict__ logits, const std::size_t pitch, const int* 
   constexpr int rows_per_wave = wave::size / G;
   const detail::columns<FULL, V, G, K> cols(experts);
   const int n = *counted;
-  const float per_token = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
-  const float scale = (grad_loss ? *grad_loss : 1.0f) * coefficient * static_cast<float>(experts) * per_token;
-  const float share = per_token / static_cast<float>(choices);
+  const double per_token = n > 0 ? 1.0 / n : 0.0;  // (factors of the whole gradient: rounded once, as products)
+  const float scale = static_cast<float>(static_cast<double>(grad_loss ? *grad_loss : 1.0f) * coefficient * experts * per_token);
+  const double share = per_token / choices;
   float weight[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int e = 0; e < V; ++e) weight[k][e] = cols.mine(k, e) ? static_cast<float>(counts[cols.at[k] + e]) * share : 0.0f;
+    for (int e = 0; e < V; ++e) weight[k][e] = cols.mine(k, e) ? static_cast<float>(counts[cols.at[k] + e] * share) : 0.0f;
   const unsigned int count = static_cast<unsigned int>(tokens);
   const unsigned int stride = gridDim.x * (4 * rows_per_wave);
   unsigned int t0 = blockIdx.x * (4 * rows_per_wave) + threadIdx.x / G;

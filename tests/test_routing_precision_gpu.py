@@ -54,3 +54,22 @@ def test_distances_beyond_every_exponent():
             f = torch.zeros(experts)
             f[0] = 1.0
             assert torch.equal(grad[0], experts * want * (f - (f * want).sum()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_factors_of_the_whole_result_are_rounded_once(dtype):
+    """Two experts of equal logits, all tokens to the first: probabilities of 1/2, f = (1, 0), every sum exact.  The loss is the coefficient
+    itself, the gradient +- upstream coefficient 2 / n / 4 rounded once (e), and once more by its store."""
+    from loops_amd import routing
+    coefficient, upstream = float(np.float32(0.3)), float(np.float32(0.7))
+    for n in [*range(1, 130), 1000, 4099, 20011, 70003]:
+        for choices in (1, 3):
+            logits = torch.zeros(n, 2, dtype=dtype, device="cuda")
+            chosen = torch.zeros(n, choices, dtype=torch.int32, device="cuda")
+            forward = routing.balance_loss(logits, chosen, coefficient=coefficient)
+            assert forward.loss.item() == coefficient and (forward.probability == 0.5).all(), (n, choices)
+            grad = routing.balance_loss_backward(logits, forward, grad_loss=torch.full((), upstream, device="cuda")).double()
+            want = upstream * coefficient * 2 / n / 4
+            store = 0.0 if dtype is torch.float32 else torch.finfo(dtype).eps / 2
+            bound = 1.01 * (E32 + store) * want + (2.0 ** -25 if dtype is torch.float16 else 0.0)
+            assert (grad[:, 0] - want).abs().max() <= bound and (grad[:, 1] + want).abs().max() <= bound, (n, choices)
