@@ -219,8 +219,8 @@ __host__ __device__ constexpr int partial_pitch(int experts) { return (experts +
 
 /**
  * Workgroup b reads tokens [b per, (b + 1) per): G lanes share a row, each keeps the sums of its own columns in registers over all of its
- * rows.  262 139 x 256 bf16 with 8 choices each: 33 us, 4.6 TB/s of logits and ids; the exponentials of a row and its reductions share the
- * time with the reads.  ONE: the only workgroup finishes as well; otherwise it leaves sums[b], counts[b] (rows of partial_pitch) and counted[b].
+ * rows.  262 139 x 256 bf16 with 8 choices each: 33 us, 4.6 TB/s of logits and ids (float: at `exponential`); the exponentials of a row and its
+ * reductions share the time with the reads.  ONE: the only workgroup finishes as well; otherwise it leaves sums[b], counts[b] (rows of partial_pitch) and counted[b].
  */
 template <bool ONE, bool FULL, int V, int G, int K, int U, typename type_t, typename id_t>
 __global__ void __launch_bounds__(threads)

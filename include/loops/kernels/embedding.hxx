@@ -48,7 +48,8 @@ constexpr int lookup_threads = 256;
  * A row is cut into `packets` = ceil(dim / V) packets of V values, the last one shifted back to end with the row (its overlap is
  * written twice, with the same values): any width and alignment moves in 16-byte accesses.  Packets of all rows are numbered through
  * and each thread takes U of them, a workgroup's width apart: consecutive lanes touch consecutive packets whatever the width.
- * HBM bounds it: 65 536 of 131 072 rows of 2 048 floats in 127 us, 5.9 TB/s; 16 tokens take 2.4 us, a launch.
+ * HBM bounds it: 65 536 tokens of a 131 072 x 2 048 float table in 125 us where ids fall off as in text (20 079 different rows: 5.6 TB/s of what
+ * has to move), 162 where they are uniform (51 665: 5.9); 16 tokens take 2.4 us, a launch.
  */
 template <int V, int U, bool STREAM, typename type_t, typename id_t>
 __global__ void __launch_bounds__(lookup_threads)
@@ -116,7 +117,7 @@ int launch_lookup(hipStream_t stream, const type_t* table, std::size_t table_pit
   using one = std::integral_constant<int, 1>;
   using width = std::integral_constant<int, V>;
   // Four packets per thread where that still fills the chip (bf16, dim 4 096: 512 tokens 3.4 us with one, 4.2 with four; 2 048: 6.6, 6.1;
-  // 16 384: 48.5, 41.0).  Stores of whole lines go past the caches (65 536 x 2 048 float: 160 us, 198 through them); others are left to the
+  // 16 384: 48.5, 41.0).  Stores of whole lines go past the caches (65 536 x 2 048 float, uniform ids: 160 us, 198 through them); others are left to the
   // L2 to gather.
   const bool whole_lines = (reinterpret_cast<std::uintptr_t>(out) | (out_pitch * sizeof(type_t)) | (dim * sizeof(type_t))) % 128 == 0;
   const bool many = static_cast<unsigned long long>(tokens) * dim >= 512ull * lookup_threads * 4 * V;
@@ -161,8 +162,11 @@ struct tile_record {
   int tail_row;
 };
 
-/// One launch instead of two is 4 us of the host's time; its own grows with the tokens (x 1 024 bf16 into float: 128 tokens 6.2 us, 7.8 with the
-/// join; 512: 12.2, 7.9; 1 024: 22.2, 8.4).
+/// A rule for calls that the host makes one by one: one launch instead of two, and no workspace, save it 4 us.  With the grouping before it a call
+/// takes 15.3 us up to 512 tokens whatever the width (64, 1 024, 8 192 columns, bf16 into float and float; 8 192: 16.8 at 512), 18.9 at 640 (21.0) and
+/// 20.0 at 768 (22.3), in two launches 19.8 at all of them.  Replayed from a graph, where the host's time is gone, the one launch is shorter up to 256
+/// tokens (x 1 024: 128 6.2 us, 7.9 with the join; 256 7.3, 8.1; 384 11.4, 8.2; 512 12.2, 8.1; 640 16.1, 8.3); the rule is the same there, as the two
+/// forms add in different orders and equal inputs give equal bits.
 constexpr int small_tokens = 640;  ///< most tokens of add_small
 
 /// Workspace: records[tiles], heads[tiles][dim], tails[tiles][dim] (float).
@@ -320,6 +324,8 @@ __device__ __forceinline__ void clear_empty(const int* __restrict__ keys, int to
  * TB/s (8 192 tokens, 131 072 rows of 8 KB: 203 us, now 172, 6.6 TB/s).
  * 8 wavefronts per SIMD are asked for: scalar registers would allow 7 otherwise (131 072 tokens x 4 096 bf16 into float, whole pass: 670
  * us, 632 with 8: 5.1 TB/s of reads and writes together, where a copy of 4 GiB reaches 4.7).
+ * ADD at the same size, 32 600 different rows: 471 us, 4.5 TB/s, the copy's rate; 8 rows in flight (475), 8 wavefronts asked for (473) and stores past
+ * the caches (470 to 475) leave it there.
  */
 template <bool ADD, int V, int U, bool STREAM, typename type_t, typename out_t>
 __global__ void __launch_bounds__(gradient_threads, ADD ? 1 : 8)
@@ -501,9 +507,9 @@ constexpr int join_waves = join_threads / wave::size;
 
 /**
  * The rows that more than one tile holds: sum of the tails of the tiles before, in a fixed order, and the finishing tile's head.
- * A workgroup covers 128 columns and every gridDim.y-th tile; its wavefronts share a row's tails out.  One CU's reads bound it (a row
- * of 10 000 of 20 011 tokens leaves 590 tails of 1 001 columns: 16 us at 256 columns per workgroup, 13 at 128, 11 at 64, where the
- * many short joins of 131 072 x 4 096 take 4 us more).
+ * A workgroup covers 128 columns and every gridDim.y-th tile; its wavefronts share a row's tails out.  A long row's tails are read by as many
+ * CUs as it has groups of columns, which bounds it (a row of 10 000 of 20 011 tokens leaves 590 tails of 1 001 columns: 16 us at 256
+ * columns per workgroup, 13 at 128, 11 at 64, where the many short joins of 131 072 x 4 096 take 4 us more).
  */
 template <bool ADD, typename out_t>
 __global__ void __launch_bounds__(join_threads)

@@ -584,7 +584,8 @@ int loops_allgatherv_f64(void* comm, int rank, int world, double* y_full, const 
  * another rank's shard of the table holds -- has a zero row in the lookup and no part in the gradient; no id is an error.
  * Calls are asynchronous and may be captured; they keep nothing between calls: scratch memory is the caller's `workspace`
  * (hipMalloc'd, 16-byte aligned, at least what the *_workspace function says for the same sizes, LOOPS_E_BADARG otherwise; it may be
- * NULL where that is 0), used by one call at a time.  tokens + rows must stay below 2^31 (LOOPS_E_RANGE). */
+ * NULL where that is 0), used by one call at a time.  Grouping and gradient: tokens + rows below 2^31 - 4 096 (LOOPS_E_RANGE).  Rows may have up
+ * to 2^31 - 1 columns; more than 2^27, or a lookup of more than 2^32 accesses, take several launches. */
 enum loops_value_type { LOOPS_VALUE_F32 = 0, LOOPS_VALUE_F16 = 1, LOOPS_VALUE_BF16 = 2 };
 enum loops_index_type { LOOPS_INDEX_I32 = 0, LOOPS_INDEX_I64 = 1 };
 
@@ -611,7 +612,7 @@ int loops_embedding_gradient(int grad_type, int out_type, int tokens, const int*
 /* ---- balance of a router ---------------------------------------------------------------------------------------------------
  * No reference counterpart.  Column sums of the routing matrix (tokens x experts, `choices` ones per row) and the loss that keeps
  * them even (include/loops/kernels/balance_loss.hxx).  Types, pitches, workspaces and capture as above.  1 <= experts <= 1024
- * (LOOPS_E_CONFIG beyond), tokens * choices < 2^31 (LOOPS_E_RANGE).  `chosen` [tokens, choices]: expert indices, packed; indices outside
+ * (LOOPS_E_CONFIG beyond), tokens * choices < 2^31 - 4 096 (LOOPS_E_RANGE).  `chosen` [tokens, choices]: expert indices, packed; indices outside
  * [0, experts) are not counted.  `mask` [tokens] (NULL: all): a token whose byte is 0 takes no part in anything and its gradient row is 0
  * (its logits may hold anything). */
 int loops_expert_counts_workspace(int tokens, int choices, int experts, size_t* bytes);
